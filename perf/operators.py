@@ -221,7 +221,7 @@ def _prepare_packed(case, seed):
     for n in lens:
         starts.append(starts[-1] + n)
     return dict(q=q, k=k, v=v, lens=lens, starts=torch.tensor(starts, dtype=torch.int32, device="cuda"),
-                longest=max(lens), causal=case["causal"], window=case["window"], cap=case["cap"],
+                causal=case["causal"], window=case["window"], cap=case["cap"],
                 slopes=_slopes(case), prefix=prefix, scale=1.0 / math.sqrt(case["head_dim"]),
                 prefix_lens=None if prefix is None else torch.tensor(prefix, dtype=torch.int32, device="cuda"))
 
@@ -386,9 +386,9 @@ def _own_pages(s):
 
 def _own_packed(s):
     from smaq_amd.exact_attention import compute_packed_attention
-    return compute_packed_attention(s["q"], s["k"], s["v"], s["starts"], s["longest"], scale=s["scale"],
-                                    causal=s["causal"], prefix_lens=s["prefix_lens"], window=s["window"],
-                                    score_cap=s["cap"], alibi_slopes=s["slopes"])
+    return compute_packed_attention(s["q"], s["k"], s["v"], s["starts"], scale=s["scale"], causal=s["causal"],
+                                     prefix_lens=s["prefix_lens"], window=s["window"], score_cap=s["cap"],
+                                    alibi_slopes=s["slopes"])
 
 
 def _own_paged(s):
