@@ -387,7 +387,7 @@ def _own_pages(s):
 def _own_packed(s):
     from smaq_amd.exact_attention import compute_packed_attention
     return compute_packed_attention(s["q"], s["k"], s["v"], s["starts"], scale=s["scale"], causal=s["causal"],
-                                     prefix_lens=s["prefix_lens"], window=s["window"], score_cap=s["cap"],
+                                    prefix_lens=s["prefix_lens"], window=s["window"], score_cap=s["cap"],
                                     alibi_slopes=s["slopes"])
 
 
