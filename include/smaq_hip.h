@@ -393,6 +393,139 @@ int smaq_attn_hybrid(const smaq_attn_params* p, void* stream);
 int smaq_attn_hybrid_noalloc(const smaq_attn_params* p, void* stream);
 
 /*
+ * The exact path around the compressed cache.  No counterparts in the
+ * reference: it takes queries and keys as a layer hands them over and serves
+ * prefill and uncompressed tokens with the host framework's own attention.
+ *
+ * Queries and keys normed per head and rotated, one pass over both:
+ *   y = x * rsqrt(mean(x^2) + eps) * (w + weight_offset)    (weight NULL: y = x)
+ *   (a, b) of pair i at position p -> (a c - b s, a s + b c),
+ *   c = gain cos(p freqs[i]), s = gain sin(p freqs[i]); pairs (i, r/2 + i) of
+ *   y[0..r), or (2i, 2i + 1) if interleaved; dims r.. are written as y.
+ * fp32 throughout, rounded once; p freqs[i] loses its whole turns in fp64.
+ * Either side may be absent (0 heads).
+ */
+typedef struct smaq_rotary_params {
+  int dtype;                 /* of q, k and both outputs */
+  int n_q_heads, n_k_heads;
+  int head_dim;              /* 1..1024 */
+  int rotary_dim;            /* r: even, 0..head_dim */
+  int interleaved;
+  long long tokens;
+  const void* q;             /* element (t, h, d) at q + t q_stride_t + h q_stride_h + d */
+  long long q_stride_t, q_stride_h;
+  const void* k;
+  long long k_stride_t, k_stride_h;
+  void* q_out;               /* [tokens][heads][head_dim], dense; no overlap with an input */
+  void* k_out;
+  const void* positions;     /* [tokens] integers of position_bytes (4 or 8) */
+  int position_bytes;
+  const double* freqs;       /* [r/2] angle per position */
+  float gain;
+  const void* q_weight;      /* [head_dim] of weight_dtype, or NULL: not normed */
+  const void* k_weight;
+  int weight_dtype;
+  float eps;
+  float weight_offset;
+} smaq_rotary_params;
+int smaq_norm_rotary(const smaq_rotary_params* p, void* stream);
+
+/*
+ * Block tables and slots of one scheduler step.  Request b holds
+ * context_lens[b] tokens and gets new_lens[b] more (negative: 0; integers of
+ * 4 or 8 bytes); the pages it needs beyond ceil(context / block_size) are
+ * taken off the front of free_blocks in request order and written into its row
+ * of block_table [requests][max_blocks] behind the ones it has.  Other entries
+ * keep their value.  The step's tokens are the requests' new ones, back to back:
+ *   slot_mapping[i] = page * block_size + offset, or -1: behind the last
+ *     token, or no page (max_blocks or the free list exceeded, or the table's
+ *     entry for a partly filled page negative; a taken column beyond the free
+ *     list gets the entry -1)
+ *   positions[i]: the token's position in its request (0 behind the last)
+ *   query_start_loc [requests + 1], seq_lens [requests] = context + new
+ *   status[0] = pages taken (more than n_free: the list was too short),
+ *   status[1] = new tokens without a slot
+ * 32-bit results stop at 2^31 - 1.  requests <= 8000.  free_blocks must be
+ * numbers of 0 or more.  Reads no length on the host: no synchronisation.
+ */
+int smaq_page_step(const void* context_lens, int context_bytes, const void* new_lens, int new_bytes,
+                   int requests, int* block_table, int max_blocks, const int* free_blocks,
+                   long long n_free, int block_size, long long tokens, long long* slot_mapping,
+                   long long* positions, int* query_start_loc, int* seq_lens, int* status, void* stream);
+
+/*
+ * Attention over a step's own exact tokens, several documents back to back.
+ * Query i and key j are positions within one document (tokens starts[b] ..
+ * starts[b+1] - 1); j is visible to i when
+ *   (not causal or j <= i or j < prefix_lens[b]) and
+ *   (window == 0 or j > i - window or j < prefix_lens[b]);
+ *   x = scale q_i.k_j;  x = score_cap tanh(x / score_cap) if score_cap > 0;
+ *   x -= alibi_slopes[head] |i - j|;  out_i = softmax_j(x) v.
+ * What lies in a place that i does not see (NaN and infinities among it) does
+ * not reach row i.  fp16 or bf16; sums and softmax in fp32, weights rounded to
+ * the values' type before their product.
+ */
+typedef struct smaq_packed_params {
+  int dtype;                 /* SMAQ_F16 or SMAQ_BF16: q, k, v, out */
+  int n_docs;
+  int n_q_heads, n_kv_heads;
+  int head_dim;              /* a multiple of 8 up to 256 */
+  int causal;
+  int window;                /* 0: none */
+  int zero_rest;             /* rows of no document: 1 written as zeros, 0 left as they are */
+  long long n_tokens;        /* rows of q, k, v and out */
+  float scale;
+  float score_cap;           /* 0: none */
+  const int* starts;         /* [n_docs + 1], ascending (numbers outside 0..n_tokens are cut) */
+  const int* prefix_lens;    /* [n_docs] or NULL */
+  const float* alibi_slopes; /* [n_q_heads] or NULL */
+  /* element (t, h, d) at x + t stride_t + h stride_h + d; pointers 16-byte
+     aligned, strides multiples of 8 */
+  const void *q, *k, *v;
+  void* out;
+  long long q_stride_t, q_stride_h, k_stride_t, k_stride_h, v_stride_t, v_stride_h, out_stride_t, out_stride_h;
+} smaq_packed_params;
+int smaq_packed_attention(const smaq_packed_params* p, void* stream);
+
+/*
+ * Attention of one new token per sequence over a paged exact cache.  The query
+ * is the sequence's last token (position seq_lens[b] - 1, its key and value
+ * already in the cache); it sees the last `window` tokens (0: all), scored as in
+ * smaq_packed_attention.  Token t of sequence b is row t % block_size of block
+ * block_table[b][t / block_size]; tokens whose entry is not a block of the cache
+ * are left out, and rows that see no token are written as zeros.  Sequences
+ * longer than max_seq_len or their table row are cut.  The length is split over
+ * workgroups and joined in split order by a second launch.
+ */
+typedef struct smaq_paged_params {
+  int dtype;                 /* SMAQ_F16 or SMAQ_BF16: q, cache, out */
+  int batch;
+  int n_q_heads, n_kv_heads;
+  int head_dim;              /* a multiple of 8 up to 256 */
+  int block_size;            /* a multiple of 16 */
+  int num_blocks;            /* blocks of the cache */
+  int max_blocks;            /* entries of a table row */
+  int window;                /* 0: none */
+  int seq_lens_wide;         /* seq_lens is int64, else int32 */
+  long long max_seq_len;     /* no sequence is longer */
+  float scale;
+  float score_cap;           /* 0: none */
+  const void* seq_lens;      /* [batch] */
+  const int* block_table;    /* [batch][max_blocks] */
+  const float* alibi_slopes; /* [n_q_heads] or NULL */
+  /* pointers 16-byte aligned, strides (elements) multiples of 8, the last dim dense */
+  const void* q;             /* [batch][n_q_heads][head_dim] */
+  const void *k_cache, *v_cache; /* [num_blocks][block_size][n_kv_heads][head_dim] */
+  void* out;                 /* [batch][n_q_heads][head_dim] */
+  long long q_stride_b, q_stride_h, out_stride_b, out_stride_h;
+  long long k_stride_block, k_stride_t, k_stride_h, v_stride_block, v_stride_t, v_stride_h;
+  void* workspace;           /* smaq_paged_workspace_bytes, 16-byte aligned */
+  long long workspace_bytes;
+} smaq_paged_params;
+long long smaq_paged_workspace_bytes(const smaq_paged_params* p);
+int smaq_paged_attention(const smaq_paged_params* p, void* stream);
+
+/*
  * Streaming-read probe.  No counterpart in the reference: a measurement
  * utility that reads `bytes` (a multiple of 16) from `src` once in 16-byte
  * loads over the whole device and writes nothing unless the XOR of

@@ -17,8 +17,11 @@ from smaq_amd.core import (AttentionBackend, CacheBackend, CacheCapabilities, Ca
                            MetricStrategy, ModelLayoutAdapter, QuantizationStrategy)
 from smaq_amd.layout import (GemmaModelLayoutAdapter, GenericModelLayoutAdapter, QwenModelLayoutAdapter,
                              infer_model_layout_adapter)
+from smaq_amd.exact_attention import compute_packed_attention, compute_paged_attention
 from smaq_amd.kv_cache import SMAQKVCache, ValueQuantized, dequantize_values, quantize_values, unpack_values
+from smaq_amd.paging import PageStep, build_page_step
 from smaq_amd.quantizer import SMAQQuantized, SMAQQuantizer
+from smaq_amd.rotary import RotaryPositions, apply_norm_rotary
 from smaq_amd.score import MIN_HISTORY_FOR_SMAQ, HybridAttentionBackend, compute_hybrid_attention
 from smaq_amd.store import CompressedKVStore, FlatCache
 from smaq_amd.strategies import (ExactShadowStrategy, IdentityMetricStrategy, IdentityScalarStrategy,

@@ -58,6 +58,49 @@ class AttnParams(ctypes.Structure):
     ]
 
 
+class RotaryParams(ctypes.Structure):
+    """Mirror of ``smaq_rotary_params`` (include/smaq_hip.h)."""
+
+    _fields_ = [
+        ("dtype", c_int), ("n_q_heads", c_int), ("n_k_heads", c_int), ("head_dim", c_int), ("rotary_dim", c_int),
+        ("interleaved", c_int), ("tokens", c_ll),
+        ("q", c_void_p), ("q_stride_t", c_ll), ("q_stride_h", c_ll),
+        ("k", c_void_p), ("k_stride_t", c_ll), ("k_stride_h", c_ll),
+        ("q_out", c_void_p), ("k_out", c_void_p), ("positions", c_void_p), ("position_bytes", c_int),
+        ("freqs", c_void_p), ("gain", c_float), ("q_weight", c_void_p), ("k_weight", c_void_p),
+        ("weight_dtype", c_int), ("eps", c_float), ("weight_offset", c_float),
+    ]
+
+
+class PackedParams(ctypes.Structure):
+    """Mirror of ``smaq_packed_params`` (include/smaq_hip.h)."""
+
+    _fields_ = [
+        ("dtype", c_int), ("n_docs", c_int), ("n_q_heads", c_int), ("n_kv_heads", c_int), ("head_dim", c_int),
+        ("causal", c_int), ("window", c_int), ("zero_rest", c_int), ("n_tokens", c_ll),
+        ("scale", c_float), ("score_cap", c_float), ("starts", c_void_p), ("prefix_lens", c_void_p),
+        ("alibi_slopes", c_void_p), ("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("out", c_void_p),
+        ("q_stride_t", c_ll), ("q_stride_h", c_ll), ("k_stride_t", c_ll), ("k_stride_h", c_ll),
+        ("v_stride_t", c_ll), ("v_stride_h", c_ll), ("out_stride_t", c_ll), ("out_stride_h", c_ll),
+    ]
+
+
+class PagedParams(ctypes.Structure):
+    """Mirror of ``smaq_paged_params`` (include/smaq_hip.h)."""
+
+    _fields_ = [
+        ("dtype", c_int), ("batch", c_int), ("n_q_heads", c_int), ("n_kv_heads", c_int), ("head_dim", c_int),
+        ("block_size", c_int), ("num_blocks", c_int), ("max_blocks", c_int), ("window", c_int),
+        ("seq_lens_wide", c_int), ("max_seq_len", c_ll), ("scale", c_float), ("score_cap", c_float),
+        ("seq_lens", c_void_p), ("block_table", c_void_p), ("alibi_slopes", c_void_p),
+        ("q", c_void_p), ("k_cache", c_void_p), ("v_cache", c_void_p), ("out", c_void_p),
+        ("q_stride_b", c_ll), ("q_stride_h", c_ll), ("out_stride_b", c_ll), ("out_stride_h", c_ll),
+        ("k_stride_block", c_ll), ("k_stride_t", c_ll), ("k_stride_h", c_ll),
+        ("v_stride_block", c_ll), ("v_stride_t", c_ll), ("v_stride_h", c_ll),
+        ("workspace", c_void_p), ("workspace_bytes", c_ll),
+    ]
+
+
 _SIGS = {
     "smaq_version": (c_int, []),
     "smaq_last_error": (ctypes.c_char_p, []),
@@ -88,6 +131,12 @@ _SIGS = {
     "smaq_attn_hybrid": (c_int, [ctypes.POINTER(AttnParams), c_void_p]),
     "smaq_attn_hybrid_noalloc": (c_int, [ctypes.POINTER(AttnParams), c_void_p]),
     "smaq_probe_read": (c_int, [c_void_p, c_ll, c_void_p, c_void_p]),
+    "smaq_norm_rotary": (c_int, [ctypes.POINTER(RotaryParams), c_void_p]),
+    "smaq_page_step": (c_int, [c_void_p, c_int, c_void_p, c_int, c_int, c_void_p, c_int, c_void_p, c_ll, c_int, c_ll,
+                               c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "smaq_packed_attention": (c_int, [ctypes.POINTER(PackedParams), c_void_p]),
+    "smaq_paged_workspace_bytes": (c_ll, [ctypes.POINTER(PagedParams)]),
+    "smaq_paged_attention": (c_int, [ctypes.POINTER(PagedParams), c_void_p]),
     "smaq_apply_values_workspace_bytes": (c_ll, [c_ll, c_ll, c_ll, c_int]),
     "smaq_apply_values": (c_int, [c_void_p, c_ll, c_ll, c_ll, c_ll, c_ll, c_int, c_void_p, c_ll, c_int, c_int,
                                   c_void_p, c_void_p, c_ll, c_int, c_void_p, c_void_p, c_ll, c_void_p]),
@@ -595,3 +644,49 @@ def attn_hybrid_noalloc(p: AttnParams, device: torch.device) -> None:
     Raises ValueError when the shapes need more than NOALLOC_SCRATCH_BYTES.
     Calls that overlap on one GPU share that workspace and race."""
     _check(lib().smaq_attn_hybrid_noalloc(ctypes.byref(p), _stream(device)), "smaq_attn_hybrid_noalloc")
+
+
+# ------------------------------------------------------------- exact path ---
+
+def require_plain(what: str, *tensors) -> None:
+    """The exact path's operators have no derivative: tensors that ask for one
+    are refused."""
+    dual = torch.autograd.forward_ad._current_level >= 0
+    for t in tensors:
+        if t is None:
+            continue
+        if (t.requires_grad and torch.is_grad_enabled()) or (
+                dual and torch.autograd.forward_ad.unpack_dual(t).tangent is not None):
+            raise ValueError(f"{what} computes no gradients: call it under torch.no_grad() or detach its inputs")
+
+
+def launch_on(dev: torch.device, fn, what: str, *args) -> None:
+    """fn(*args, stream) on the device's current stream, with that device current."""
+    if torch.cuda.current_device() == dev.index:
+        _check(fn(*args, _stream(dev)), what)
+        return
+    with torch.cuda.device(dev):
+        _check(fn(*args, _stream(dev)), what)
+
+
+def rows_aligned(t: torch.Tensor, lead: int) -> bool:
+    """Whether the last dim is dense and every row of 16-bit elements starts on
+    16 bytes (the first ``lead`` dims' strides are multiples of 8)."""
+    return (t.stride(-1) == 1 and t.data_ptr() % 16 == 0
+            and all(st % 8 == 0 or n == 1 for n, st in zip(t.shape[:lead], t.stride()[:lead])))
+
+
+def strides(t: torch.Tensor, lead: int) -> list:
+    """The first ``lead`` strides, 0 where a dim has one entry."""
+    return [0 if n == 1 else st for n, st in zip(t.shape[:lead], t.stride()[:lead])]
+
+
+def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the address ranges of two tensors meet."""
+    def span(t):
+        if t.numel() == 0:
+            return 0, 0
+        reach = sum((n - 1) * st for n, st in zip(t.shape, t.stride())) + 1
+        return t.data_ptr(), t.data_ptr() + reach * t.element_size()
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1

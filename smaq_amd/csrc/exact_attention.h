@@ -1,0 +1,48 @@
+// What the two attention kernels over exact keys share (not part of the C ABI).
+#pragma once
+
+#include "smaq_common.h"
+
+namespace smaq {
+
+constexpr float kLog2eF = 1.4426950408889634f;
+
+// Scores in units of log2: scale, tanh cap and distance bias as the kernels apply
+// them to a product q.k.
+struct ScoreRule {
+  float scale;  // no cap: scale log2(e); cap: 2 log2(e) scale / cap
+  float cap;    // cap log2(e); 0: none
+  int wide;     // the cap is above kWideCap
+};
+
+// cap (1 - 2 / (e^(2x/cap) + 1)) loses what lies below some 2^-22 of the cap: up to
+// this cap that moves a weight by less than 2^-13 (half a step of fp16 is 2^-11);
+// above it small arguments take the series of tanh.
+constexpr float kWideCap = 256.0f;
+
+// Whether rows of 16-bit elements start on 16 bytes.
+template <typename... S>
+inline bool rows_on_16(const void* p, S... strides) {
+  return (uintptr_t)p % 16 == 0 && ((strides % 8 == 0) && ...);
+}
+
+inline ScoreRule score_rule(float scale, float cap) {
+  if (cap > 0.0f)
+    return {(float)(2.0 * 1.4426950408889634 * (double)scale / (double)cap), cap * kLog2eF, cap > kWideCap};
+  return {scale * kLog2eF, 0.0f, 0};
+}
+
+// cap tanh(x / cap) of x = scale dot, times log2(e).  The limits at +-inf are exact,
+// NaN passes.
+__device__ __forceinline__ float rule_score(const ScoreRule& r, float dot) {
+  const float x = dot * r.scale;
+  if (r.cap == 0.0f) return x;
+  const float t = fmaf(-2.0f * r.cap, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x) + 1.0f), r.cap);
+  if (!r.wide) return t;
+  // y = x / (2 log2 e): y - y^3/3 + 2 y^5/15 - 17 y^7/315 + 62 y^9/2835, below 0.35 to 2^-21
+  const float y = x * (0.5f / kLog2eF), z = y * y;
+  const float s = fmaf(z, fmaf(z, fmaf(z, 62.0f / 2835.0f, -17.0f / 315.0f), 2.0f / 15.0f), -1.0f / 3.0f);
+  return fabsf(y) < 0.35f ? r.cap * fmaf(y * z, s, y) : t;
+}
+
+}  // namespace smaq

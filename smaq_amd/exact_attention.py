@@ -1,0 +1,189 @@
+"""Attention over exact keys and values, next to the compressed history's.
+
+``compute_hybrid_attention`` and the paged pools answer a decode step from
+compressed tokens.  Around them a serving program attends exact ones: a
+prefill over the step's own tokens, several requests back to back, and decode
+over an exact paged cache (layers kept exact, contexts too short to compress).
+Scores may be capped by a tanh and biased by distance; documents, prefixes and
+windows mask them.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Optional
+
+import torch
+
+from smaq_amd import _native
+
+
+def _scores(what: str, head_dim: int, scale: Optional[float], score_cap: float, window: int):
+    scale = 1.0 / math.sqrt(head_dim) if scale is None else float(scale)
+    if not math.isfinite(scale):
+        raise ValueError(f"{what}: scale must be finite, got {scale}")
+    if not (0.0 <= score_cap < 1e30):
+        raise ValueError(f"{what}: score_cap must be 0 (none) or a finite number above it, got {score_cap}")
+    if window < 0 or window > 0x7fffffff:
+        raise ValueError(f"{what}: window must be 0 (none) or a number of tokens, got {window}")
+    return scale, float(score_cap), int(window)
+
+
+def _slopes(what: str, alibi_slopes: Optional[torch.Tensor], heads: int):
+    if alibi_slopes is None:
+        return None
+    if tuple(alibi_slopes.shape) != (heads,) or not alibi_slopes.dtype.is_floating_point:
+        raise ValueError(f"{what}: alibi_slopes must be [{heads}] floating point, got {tuple(alibi_slopes.shape)} "
+                         f"{alibi_slopes.dtype}")
+    return alibi_slopes.to(torch.float32).contiguous()
+
+
+def _heads(what: str, q: torch.Tensor, hkv: int, D: int) -> None:
+    if q.dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError(f"{what}: float16 or bfloat16 queries, keys and values, got {q.dtype}")
+    if D % 8 or not 0 < D <= 256:
+        raise ValueError(f"{what}: head_dim must be a multiple of 8 up to 256, got {D}")
+    if hkv <= 0 or q.shape[1] <= 0 or q.shape[1] % hkv:
+        raise ValueError(f"{what}: {q.shape[1]} query heads are not a multiple of {hkv} key-value heads")
+
+
+def _out(what: str, out: Optional[torch.Tensor], q: torch.Tensor, *others: torch.Tensor) -> torch.Tensor:
+    if out is None:
+        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if (out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous()
+            or out.data_ptr() % 16):
+        raise ValueError(f"{what}: out must be a contiguous, 16-byte aligned {tuple(q.shape)} {q.dtype} tensor on "
+                         f"{q.device}")
+    if any(_native.overlap(out, t) for t in (q, *others)):
+        raise ValueError(f"{what}: out shares memory with an input")
+    return out
+
+
+def compute_packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, *,
+                             scale: Optional[float] = None, causal: bool = True,
+                             prefix_lens: Optional[torch.Tensor] = None, window: int = 0, score_cap: float = 0.0,
+                             alibi_slopes: Optional[torch.Tensor] = None,
+                             out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of queries [T, Hq, D] over the same tokens' keys and values
+    [T, Hkv, D], documents back to back: document b is tokens ``cu_seqlens[b]``
+    to ``cu_seqlens[b + 1] - 1`` (integers, [documents + 1], ascending).
+
+    Within a document, row i sees key j when ``not causal or j <= i`` and
+    ``window == 0 or j > i - window``; the document's first ``prefix_lens[b]``
+    keys are seen from all its rows.  Scores are ``scale q.k`` (scale None:
+    1/sqrt(D)), then ``score_cap tanh(x / score_cap)`` if the cap is not 0, then
+    minus ``alibi_slopes[head] |i - j|``.  Whatever stands in unseen places does
+    not reach a row, NaN and infinities among it.
+
+    fp16 or bf16, head_dim a multiple of 8 up to 256; views of a packed
+    projection are read in place.  Rows of no document are zeros in a new
+    result, and left as they are in ``out``.
+    """
+    what = "compute_packed_attention"
+    dev = _native.require_gpu(q, k, v, cu_seqlens, prefix_lens, alibi_slopes, out)
+    _native.require_plain(what, q, k, v, alibi_slopes, out)
+    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]:
+        raise ValueError(f"{what}: queries [T, Hq, D] and keys and values [T, Hkv, D] expected, got {tuple(q.shape)}, "
+                         f"{tuple(k.shape)}, {tuple(v.shape)}")
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError(f"{what}: one dtype for queries, keys and values, got {q.dtype}, {k.dtype}, {v.dtype}")
+    T, Hq, D = q.shape
+    _heads(what, q, k.shape[1], D)
+    scale, cap, window = _scores(what, D, scale, score_cap, window)
+    if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1 or cu_seqlens.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{what}: cu_seqlens must be int32 or int64 [documents + 1], got {tuple(cu_seqlens.shape)} "
+                         f"{cu_seqlens.dtype}")
+    docs = cu_seqlens.numel() - 1
+    starts = cu_seqlens.to(torch.int32).contiguous()
+    if prefix_lens is not None:
+        if tuple(prefix_lens.shape) != (docs,) or prefix_lens.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"{what}: prefix_lens must be int32 or int64 [{docs}], got {tuple(prefix_lens.shape)} "
+                             f"{prefix_lens.dtype}")
+        prefix_lens = prefix_lens.to(torch.int32).contiguous()
+    slopes = _slopes(what, alibi_slopes, Hq)
+    res = _out(what, out, q, k, v)
+    q, k, v = (t if _native.rows_aligned(t, 2) else t.clone(memory_format=torch.contiguous_format) for t in (q, k, v))
+    p = _native.PackedParams()
+    p.dtype, p.n_docs, p.n_tokens = _native.dtype_code(q.dtype), docs, T
+    p.n_q_heads, p.n_kv_heads, p.head_dim = Hq, k.shape[1], D
+    p.causal, p.window, p.zero_rest, p.scale, p.score_cap = int(bool(causal)), window, int(out is None), scale, cap
+    p.starts = starts.data_ptr()
+    p.prefix_lens = None if prefix_lens is None else prefix_lens.data_ptr()
+    p.alibi_slopes = None if slopes is None else slopes.data_ptr()
+    p.q, p.k, p.v, p.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), res.data_ptr()
+    p.q_stride_t, p.q_stride_h = _native.strides(q, 2)
+    p.k_stride_t, p.k_stride_h = _native.strides(k, 2)
+    p.v_stride_t, p.v_stride_h = _native.strides(v, 2)
+    p.out_stride_t, p.out_stride_h = _native.strides(res, 2)
+    _native.launch_on(dev, _native.lib().smaq_packed_attention, "smaq_packed_attention", ctypes.byref(p))
+    return res
+
+
+def compute_paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+                            seq_lens: torch.Tensor, max_seq_len: int, *, scale: Optional[float] = None,
+                            window: int = 0, score_cap: float = 0.0, alibi_slopes: Optional[torch.Tensor] = None,
+                            out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of one new token per sequence, queries [B, Hq, D], over a paged
+    exact cache: keys and values [blocks, block_size, Hkv, D] (views such as
+    ``kv_cache[0]`` and ``kv_cache[1]`` of a flash-layout cache), token t of
+    sequence b in row ``t % block_size`` of block ``block_table[b, t // block_size]``.
+
+    The query is the sequence's last token, number ``seq_lens[b] - 1``; its key
+    and value are in the cache.  It sees the last ``window`` tokens (0: all),
+    scored as in ``compute_packed_attention``.  ``max_seq_len`` bounds every
+    length (longer sequences are cut to it) and sets how the length is split over
+    the card.  Tokens whose table entry is no block of the cache are left out; a
+    sequence without a token gives zeros.
+
+    fp16 or bf16, head_dim a multiple of 8 up to 256, block_size a multiple of
+    16, cache rows on 16 bytes.
+    """
+    what = "compute_paged_attention"
+    dev = _native.require_gpu(q, k_cache, v_cache, block_table, seq_lens, alibi_slopes, out)
+    _native.require_plain(what, q, k_cache, v_cache, alibi_slopes, out)
+    if q.dim() != 3 or k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.shape[3] != q.shape[2]:
+        raise ValueError(f"{what}: queries [B, Hq, D] and caches [blocks, block_size, Hkv, D] expected, got "
+                         f"{tuple(q.shape)}, {tuple(k_cache.shape)}, {tuple(v_cache.shape)}")
+    if k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
+        raise ValueError(f"{what}: one dtype for queries and caches, got {q.dtype}, {k_cache.dtype}, {v_cache.dtype}")
+    B, Hq, D = q.shape
+    blocks, bs, hkv, _ = k_cache.shape
+    _heads(what, q, hkv, D)
+    scale, cap, window = _scores(what, D, scale, score_cap, window)
+    if bs <= 0 or bs % 16:
+        raise ValueError(f"{what}: block_size must be a multiple of 16, got {bs}")
+    if not (_native.rows_aligned(k_cache, 3) and _native.rows_aligned(v_cache, 3)):
+        raise ValueError(f"{what}: cache rows must be dense and start on 16 bytes")
+    if block_table.dim() != 2 or block_table.shape[0] < B or block_table.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{what}: block_table must be an integer [>= {B}, max_blocks] tensor, got "
+                         f"{tuple(block_table.shape)} {block_table.dtype}")
+    if seq_lens.dim() != 1 or seq_lens.shape[0] < B or seq_lens.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{what}: seq_lens must be int32 or int64 [>= {B}], got {tuple(seq_lens.shape)} "
+                         f"{seq_lens.dtype}")
+    if max_seq_len < 0:
+        raise ValueError(f"{what}: max_seq_len must be 0 or more, got {max_seq_len}")
+    slopes = _slopes(what, alibi_slopes, Hq)
+    res = _out(what, out, q, k_cache, v_cache)
+    if not _native.rows_aligned(q, 2):
+        q = q.clone(memory_format=torch.contiguous_format)
+    table, lens = block_table[:B].to(torch.int32).contiguous(), seq_lens[:B].contiguous()
+    p = _native.PagedParams()
+    p.dtype, p.batch, p.n_q_heads, p.n_kv_heads, p.head_dim = _native.dtype_code(q.dtype), B, Hq, hkv, D
+    p.block_size, p.num_blocks, p.max_blocks, p.window = bs, blocks, table.shape[1], window
+    p.seq_lens_wide, p.max_seq_len, p.scale, p.score_cap = int(lens.dtype == torch.int64), int(max_seq_len), scale, cap
+    p.seq_lens, p.block_table = lens.data_ptr(), table.data_ptr()
+    p.alibi_slopes = None if slopes is None else slopes.data_ptr()
+    p.q, p.k_cache, p.v_cache, p.out = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), res.data_ptr()
+    p.q_stride_b, p.q_stride_h = _native.strides(q, 2)
+    p.out_stride_b, p.out_stride_h = _native.strides(res, 2)
+    p.k_stride_block, p.k_stride_t, p.k_stride_h = _native.strides(k_cache, 3)
+    p.v_stride_block, p.v_stride_t, p.v_stride_h = _native.strides(v_cache, 3)
+    lib = _native.lib()
+    size = lib.smaq_paged_workspace_bytes(ctypes.byref(p))
+    if size < 0:
+        _native._check(-1, "smaq_paged_attention")
+    ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+    p.workspace, p.workspace_bytes = (None if ws is None else ws.data_ptr()), size
+    _native.launch_on(dev, lib.smaq_paged_attention, "smaq_paged_attention", ctypes.byref(p))
+    return res

@@ -1,0 +1,73 @@
+"""Block tables and slots of a scheduler step, built on the GPU.
+
+The paged caches of this package (``PagedQuantizedKV``, the vLLM adapter's
+pools) are addressed by a block table and written by a slot map; this builds
+both from the requests' lengths without reading one back to the host.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from typing import NamedTuple
+
+import torch
+
+from smaq_amd import _native
+
+
+class PageStep(NamedTuple):
+    slot_mapping: torch.Tensor     # int64 [num_tokens], -1: no slot
+    positions: torch.Tensor        # int64 [num_tokens]
+    query_start_loc: torch.Tensor  # int32 [requests + 1]
+    seq_lens: torch.Tensor         # int32 [requests]
+    status: torch.Tensor           # int32 [2]: pages taken, new tokens without a slot
+
+
+def build_page_step(context_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tensor,
+                    free_blocks: torch.Tensor, block_size: int, num_tokens: int) -> PageStep:
+    """Pages for ``new_lens[b]`` new tokens behind the ``context_lens[b]`` that
+    request b has in the cache, and the new tokens' slots and positions.
+
+    Request b's missing pages are taken off the front of ``free_blocks`` (int32,
+    ids of 0 or more), in request order, and written into its row of
+    ``block_table`` (int32 [requests, max_blocks], contiguous, updated in place:
+    nothing but the taken entries changes, so the same call again gives the same
+    result).  ``num_tokens`` sizes the token outputs: at least the sum of
+    ``new_lens``, more for a padded step; places behind the last token get slot
+    -1 and position 0.  A token without a page (the free list or the row too
+    short, the entry of a partly filled page negative) gets slot -1 and is
+    counted in ``status[1]``; ``status[0]`` is the number of pages the step takes
+    off the list, more than it holds when it was too short.
+    """
+    dev = _native.require_gpu(context_lens, new_lens, block_table, free_blocks)
+    for t, what in ((context_lens, "context_lens"), (new_lens, "new_lens")):
+        if t.dim() != 1 or t.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"build_page_step: {what} must be a one-dimensional int32 or int64 tensor, got "
+                             f"{tuple(t.shape)} {t.dtype}")
+    n = context_lens.shape[0]
+    if new_lens.shape[0] != n:
+        raise ValueError(f"build_page_step: {new_lens.shape[0]} new lengths for {n} requests")
+    if (block_table.dim() != 2 or block_table.shape[0] < n or block_table.dtype != torch.int32
+            or not block_table.is_contiguous()):
+        raise ValueError(f"build_page_step: block_table must be a contiguous int32 [>= {n}, max_blocks] tensor, got "
+                         f"{tuple(block_table.shape)} {block_table.dtype}")
+    if free_blocks.dim() != 1 or free_blocks.dtype != torch.int32:
+        raise ValueError(f"build_page_step: free_blocks must be a one-dimensional int32 tensor, got "
+                         f"{tuple(free_blocks.shape)} {free_blocks.dtype}")
+    for t, what in ((context_lens, "context_lens"), (new_lens, "new_lens"), (free_blocks, "free_blocks")):
+        if _native.overlap(block_table, t):
+            raise ValueError(f"build_page_step: block_table shares memory with {what}")
+    ctx, new, free = context_lens.contiguous(), new_lens.contiguous(), free_blocks.contiguous()
+    num_tokens = int(num_tokens)
+    if num_tokens < 0:
+        raise ValueError(f"build_page_step: num_tokens must be 0 or more, got {num_tokens}")
+    step = PageStep(torch.empty(num_tokens, dtype=torch.int64, device=dev),
+                    torch.empty(num_tokens, dtype=torch.int64, device=dev),
+                    torch.empty(n + 1, dtype=torch.int32, device=dev), torch.empty(n, dtype=torch.int32, device=dev),
+                    torch.empty(2, dtype=torch.int32, device=dev))
+    ptr = ctypes.c_void_p
+    _native.launch_on(dev, _native.lib().smaq_page_step, "smaq_page_step", ptr(ctx.data_ptr()), ctx.element_size(),
+                      ptr(new.data_ptr()), new.element_size(), n, ptr(block_table.data_ptr()), block_table.shape[1],
+                      ptr(free.data_ptr()), free.shape[0], int(block_size), num_tokens,
+                      *(ptr(t.data_ptr()) for t in step))
+    return step
