@@ -45,4 +45,54 @@ __device__ __forceinline__ float rule_score(const ScoreRule& r, float dot) {
   return fabsf(y) < 0.35f ? r.cap * fmaf(y * z, s, y) : t;
 }
 
+// ------------------------------------------------------- matrix operands ---
+typedef float f32x4v __attribute__((ext_vector_type(4)));
+typedef float f32x16v __attribute__((ext_vector_type(16)));
+typedef float f32x2v __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4v __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2v __attribute__((ext_vector_type(2)));
+
+template <typename T>
+struct Mat;
+
+template <>
+struct Mat<_Float16> {
+  typedef _Float16 v8 __attribute__((ext_vector_type(8)));
+  typedef _Float16 v2 __attribute__((ext_vector_type(2)));
+  static __device__ __forceinline__ f32x4v mma16(u32x4v a, u32x4v b, f32x4v c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f32x16v mma32(u32x4v a, u32x4v b, f32x16v c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
+  }
+  // two numbers rounded to nearest, packed
+  static __device__ __forceinline__ uint32_t pack(float x, float y) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2v){x, y}, v2));
+  }
+};
+
+template <>
+struct Mat<bf16> {
+  typedef __bf16 v8 __attribute__((ext_vector_type(8)));
+  typedef __bf16 v2 __attribute__((ext_vector_type(2)));
+  static __device__ __forceinline__ f32x4v mma16(u32x4v a, u32x4v b, f32x4v c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f32x16v mma32(u32x4v a, u32x4v b, f32x16v c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ uint32_t pack(float x, float y) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2v){x, y}, v2));
+  }
+};
+
+// 16-bit halves of two words: (low x, low y) or (high x, high y)
+__device__ __forceinline__ uint32_t low_halves(uint32_t x, uint32_t y) { return __builtin_amdgcn_perm(y, x, 0x05040100u); }
+__device__ __forceinline__ uint32_t high_halves(uint32_t x, uint32_t y) { return __builtin_amdgcn_perm(y, x, 0x07060302u); }
+
+constexpr float kNegInf = -__builtin_inff();
+// A softmax's reference maximum is raised when a score is this much (log2) above it:
+// weights stay below 2^8, far inside fp16, and sums and outputs are rarely rescaled.
+constexpr float kRaise = 8.0f;
+
 }  // namespace smaq
