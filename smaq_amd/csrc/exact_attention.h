@@ -57,6 +57,7 @@ struct Mat;
 
 template <>
 struct Mat<_Float16> {
+  static constexpr uint32_t kExp = 0x7c00;  // exponent bits
   typedef _Float16 v8 __attribute__((ext_vector_type(8)));
   typedef _Float16 v2 __attribute__((ext_vector_type(2)));
   static __device__ __forceinline__ f32x4v mma16(u32x4v a, u32x4v b, f32x4v c) {
@@ -73,6 +74,7 @@ struct Mat<_Float16> {
 
 template <>
 struct Mat<bf16> {
+  static constexpr uint32_t kExp = 0x7f80;
   typedef __bf16 v8 __attribute__((ext_vector_type(8)));
   typedef __bf16 v2 __attribute__((ext_vector_type(2)));
   static __device__ __forceinline__ f32x4v mma16(u32x4v a, u32x4v b, f32x4v c) {
@@ -85,6 +87,12 @@ struct Mat<bf16> {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2v){x, y}, v2));
   }
 };
+
+// ones over the halves of a word of two numbers that are infinite or NaN
+template <uint32_t EXP>
+__device__ __forceinline__ uint32_t not_finite_halves(uint32_t w) {
+  return ((w & EXP) == EXP ? 0xffffu : 0u) | ((w & (EXP << 16)) == (EXP << 16) ? 0xffff0000u : 0u);
+}
 
 // 16-bit halves of two words: (low x, low y) or (high x, high y)
 __device__ __forceinline__ uint32_t low_halves(uint32_t x, uint32_t y) { return __builtin_amdgcn_perm(y, x, 0x05040100u); }

@@ -1,66 +1,382 @@
 // Attention over a step's own exact tokens (smaq_packed_attention).
+//
+// 4 D operations per visible pair and head over a few bytes per token: the matrix
+// cores bound it, then the vector unit (the exponentials) and LDS (operand reads).
+//
+// A unit of work is 32 tokens of one query head; a workgroup's four waves take four
+// units of one KV head, heads before tokens, so that they read the same keys (with
+// four heads or more on a KV head, exactly the same).  Token blocks are cut from the
+// packed rows, not from the documents: rows carry their own visible ranges, many
+// short documents share a block, and no block needs to be looked up.  A row sees at
+// most two ranges, [lo, hi) and a prefix apart from it.
+//
+//   S^T[key][q] = K . Q^T      A = K rows from LDS, B = Q in registers
+//   softmax per column q       a lane holds half the keys of its column
+//   O^T[dim][q] += V^T . P^T   B = P^T straight from the S^T accumulators (the
+//                              k-elements of half h are keys 4 h .. 4 h + 3 and
+//                              8 + 4 h ..), A = V^T by transposing LDS reads
+//
+// Tiles of 64 keys (32 at 256 dims) are copied global -> LDS one tile ahead, 16-byte
+// units placed by an XOR of the row so that operand reads meet no bank twice.
+//
+// Masks.  A tile that every row of a wave sees whole takes no mask.  In others a
+// masked score becomes -inf after scale, cap and bias, so NaN there is dropped; a
+// masked value that is not finite would still make 0 * NaN in the product.  That
+// shows as a result that is not finite: such a workgroup runs again with the masked
+// tiles' numbers that are not finite taken out of the product (the other rows keep
+// their bits) and added key by key to the rows that see them.
+#include <math.h>
+
+#include <type_traits>
+
 #include "exact_attention.h"
 
 namespace smaq {
 namespace {
 
-constexpr int kWaves = 4;
+constexpr int kThreads = 256;
+constexpr int kIntMax = 0x7fffffff;
 
-// One wave per (token, query head).
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+__device__ const u32x4v kZeroUnit = {0, 0, 0, 0};
+
+// Layout of a tile row of DT dims in LDS: 16-byte unit u of row r sits at u ^ swizzle.
+// Keys are read 32 rows x one unit, values 8 rows x 4 units at a time.
+template <int DT>
+__device__ __forceinline__ int key_swizzle(int r) { return DT == 64 ? (r >> 1) & 7 : r & 15; }
+template <int DT>
+__device__ __forceinline__ int val_swizzle(int r) { return DT == 64 ? 4 * ((r >> 1) & 1) : 4 * (r & 3); }
+
+// the last i of the ascending s[0..n) with s[i] <= x, 0 if there is none; by the wave
+__device__ __forceinline__ int wave_last(const int* s, int n, int x, int lane) {
+  int lo = 0, len = n;
+  while (len > 1) {
+    const int step = (len + 63) / 64, i = lane * step;
+    const unsigned long long at = __ballot(i < len && s[lo + min(i, len - 1)] <= x);
+    const int below = (int)__popcll(at);  // signed: none may be
+    const int pos = below > 0 ? (below - 1) * step : 0;
+    lo += pos;
+    len = min(step, len - pos);
+  }
+  return lo;
+}
+
+__device__ __forceinline__ int wave_min(int v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o, 64));
+  return __builtin_amdgcn_readfirstlane(v);
+}
+__device__ __forceinline__ int wave_max(int v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = max(v, __shfl_xor(v, o, 64));
+  return __builtin_amdgcn_readfirstlane(v);
+}
+
+template <typename T, int DT, bool CAP, bool ALIBI>
+__global__ __launch_bounds__(kThreads, 2) void packed_kernel(smaq_packed_params p, ScoreRule rule, int blocks) {
+  constexpr int KT = DT == 256 ? 32 : 64;  // keys per tile
+  constexpr int KB = KT / 32;              // 32-key blocks
+  constexpr int KS = DT / 16;              // k steps of a product over the head dim
+  constexpr int DB = DT / 32;              // 32-dim blocks of the output
+  constexpr int UPR = DT / 8;              // 16-byte units of a row
+  constexpr int RS = DT * 2;               // bytes of a row
+  constexpr int TILE = KT * RS;            // bytes of a key or value tile
+  constexpr int LOADS = KT * UPR / kThreads;
+  __shared__ __attribute__((aligned(16))) char lds[4 * TILE];  // two buffers of (keys, values)
+  __shared__ int span[4][4];
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, half = lane >> 5;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int g = p.n_q_heads / p.n_kv_heads, D = p.head_dim, T_all = (int)p.n_tokens;
+  const int h = blockIdx.x % p.n_kv_heads;
+  // the last tokens first: with a causal mask they have the most keys
+  const int groups = (blocks * g + 3) / 4;
+  const int unit = 4 * (groups - 1 - (int)(blockIdx.x / p.n_kv_heads)) + w;
+  const int tb = unit / g, hq = h * g + unit % g;
+  const int row = 32 * tb + n;
+
+  // ---- the ranges of this lane's row: [lo, hi), and [lo2, hi2) if the prefix is apart
+  int lo = 0, hi = 0, lo2 = 0, hi2 = 0;
+  if (unit < blocks * g && p.n_docs > 0) {
+    const int t0 = 32 * tb, t1 = min(t0 + 31, T_all - 1);
+    int d = wave_last(p.starts, p.n_docs, t0, lane);
+    const int d1 = wave_last(p.starts, p.n_docs, t1, lane);
+    for (int end = d1 + 1; end - d > 1;) {
+      const int mid = (d + end) >> 1;
+      if (p.starts[mid] <= row) d = mid; else end = mid;
+    }
+    const int s = max(p.starts[d], 0), e = min(p.starts[d + 1], T_all);
+    if (row >= s && row < e) {
+      lo = p.window ? max(s, row - p.window + 1) : s;
+      hi = p.causal ? row + 1 : e;
+      const int pre = p.prefix_lens ? s + min(max(p.prefix_lens[d], 0), e - s) : s;
+      if (pre >= lo) {
+        lo = s;
+        hi = max(hi, pre);
+      } else if (pre > s) {
+        lo2 = s;
+        hi2 = pre;
+      }
+    }
+  }
+  const bool live = hi > lo;
+  const bool apart = hi2 > lo2;
+  // of the wave: first and last key, the gap no row looks into, the keys all rows see
+  const int w_lo = wave_min(live ? (apart ? lo2 : lo) : kIntMax), w_hi = wave_max(live ? hi : 0);
+  const int w_gap0 = wave_max(apart ? hi2 : (live ? lo : 0)), w_gap1 = wave_min(live ? lo : kIntMax);
+  const int w_full0 = wave_max(live ? lo : 0), w_full1 = wave_min(live ? hi : kIntMax);
+  if (lane == 0) {
+    span[w][0] = w_lo;
+    span[w][1] = w_hi;
+    span[w][2] = w_gap0;
+    span[w][3] = w_gap1;
+  }
+  __syncthreads();
+  int k_lo = kIntMax, k_hi = 0, gap0 = 0, gap1 = kIntMax;
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    k_lo = min(k_lo, __builtin_amdgcn_readfirstlane(span[x][0]));
+    k_hi = max(k_hi, __builtin_amdgcn_readfirstlane(span[x][1]));
+    gap0 = max(gap0, __builtin_amdgcn_readfirstlane(span[x][2]));
+    gap1 = min(gap1, __builtin_amdgcn_readfirstlane(span[x][3]));
+  }
+
+  // ---- queries: column n, dims 16 ks + 8 half ..; a negative scale is taken into them
+  u32x4v qr[KS];
+  {
+    const T* src = (const T*)p.q + (int64_t)row * p.q_stride_t + hq * p.q_stride_h;
+    const uint32_t flip = p.scale < 0.0f ? 0x80008000u : 0u;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      qr[ks] = u32x4v{0, 0, 0, 0};
+      if (live && 16 * ks + 8 * half < D) qr[ks] = *(const u32x4v*)(src + 16 * ks + 8 * half) ^ flip;
+    }
+  }
+  const float slope = ALIBI ? (live ? p.alibi_slopes[hq] * kLog2eF : 0.0f) : 0.0f;
+
+  // ---- tile copies: load i of thread tid fills unit 256 i + tid of the tile
+  const T* kc = (const T*)p.k + h * p.k_stride_h;
+  const T* vc = (const T*)p.v + h * p.v_stride_h;
+  auto copy_tile = [&](int k, int buf) {
+    char* kd = lds + buf * 2 * TILE;
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int r = (kThreads * i + tid) / UPR, u = tid % UPR;
+      const int64_t key = min(k + r, k_hi - 1);
+      const int uk = u ^ key_swizzle<DT>(r), uv = u ^ val_swizzle<DT>(r);
+      const void* ks = 8 * uk < D ? (const void*)(kc + key * p.k_stride_t + 8 * uk) : (const void*)&kZeroUnit;
+      const void* vs = 8 * uv < D ? (const void*)(vc + key * p.v_stride_t + 8 * uv) : (const void*)&kZeroUnit;
+      __builtin_amdgcn_global_load_lds(ks, (__attribute__((address_space(3))) void*)(kd + 16 * (kThreads * i + 64 * w)), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds(vs, (__attribute__((address_space(3))) void*)(kd + TILE + 16 * (kThreads * i + 64 * w)), 16, 0, 0);
+    }
+  };
+  // the tile behind k: the next keys, or past the gap
+  auto next_tile = [&](int k) {
+    k += KT;
+    return k >= gap0 && k + KT <= gap1 && gap1 < k_hi ? gap1 : k;
+  };
+
+  // ---- operand addresses within a tile
+  const int krow = n * RS;
+  int koff[KS];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) koff[ks] = krow + 16 * ((2 * ks + half) ^ key_swizzle<DT>(n));
+  const int vr0 = 4 * half + ((lane & 15) >> 2);
+  int voff[DB < 4 ? DB : 4];
+#pragma unroll
+  for (int db = 0; db < (DB < 4 ? DB : 4); ++db)
+    voff[db] = vr0 * RS + 16 * ((4 * db + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) ^ val_swizzle<DT>(vr0)) + 8 * (lane & 1);
+
+  f32x16v acc[DB];
+  float m_ref, m_use, m_thr, l;
+  auto run = [&](auto careful_tag) {
+    constexpr bool careful = decltype(careful_tag)::value;
+#pragma unroll
+    for (int db = 0; db < DB; ++db) acc[db] = f32x16v{};
+    m_ref = m_thr = kNegInf;
+    m_use = l = 0.0f;
+    if (k_lo < k_hi) copy_tile(k_lo, 0);
+    int buf = 0;
+    for (int k = k_lo; k < k_hi; buf ^= 1) {
+      // this thread's copies have landed, then everyone's; everyone is done with the
+      // other buffer
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_s_waitcnt(0);
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      const int k_next = next_tile(k);
+      if (k_next < k_hi) copy_tile(k_next, buf ^ 1);
+      const int k0 = k;
+      k = k_next;
+      if (k0 >= w_hi || k0 + KT <= w_lo || (k0 >= w_gap0 && k0 + KT <= w_gap1)) continue;
+      const char* kt = lds + buf * 2 * TILE;
+      const char* vt = kt + TILE;
+      f32x16v s[KB];
+      __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        s[kb] = f32x16v{};
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+          s[kb] = Mat<T>::mma32(*(const u32x4v*)(kt + koff[ks] + kb * 32 * RS), qr[ks], s[kb]);
+      }
+      __builtin_amdgcn_s_setprio(0);
+      // key of register i of block kb: k0 + 32 kb + 8 (i / 4) + 4 half + i % 4
+      const bool full = k0 >= w_full0 && k0 + KT <= w_full1;
+      const float gap = ALIBI ? (float)(row - k0 - 4 * half) : 0.0f;
+      uint32_t pk[KB][8];
+      auto weights = [&](auto masked) {
+        constexpr bool MASK = decltype(masked)::value;
+        float mx = kNegInf;
+        if constexpr (MASK || ALIBI) {
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              float x = CAP ? rule_score(rule, s[kb][i]) : s[kb][i] * rule.scale;
+              if constexpr (ALIBI) x = fmaf(-slope, fabsf(gap - (float)(32 * kb + 8 * (i / 4) + i % 4)), x);
+              if constexpr (MASK) {
+                const int key = k0 + 4 * half + 32 * kb + 8 * (i / 4) + i % 4;
+                x = (key >= lo && key < hi) || (key >= lo2 && key < hi2) ? x : kNegInf;
+              }
+              s[kb][i] = x;
+              mx = fmaxf(mx, x);
+            }
+        } else {
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kb][i]);
+          mx = CAP ? rule_score(rule, mx) : mx * rule.scale;
+        }
+        if (__any(mx > m_thr)) {
+          mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+          const float m_new = fmaxf(m_ref, mx);
+          m_use = m_new == kNegInf ? 0.0f : m_new;
+          const float alpha = __builtin_amdgcn_exp2f(m_ref - m_use);
+          l *= alpha;
+#pragma unroll
+          for (int db = 0; db < DB; ++db) acc[db] *= alpha;
+          m_ref = m_new;
+          m_thr = m_new + kRaise;
+        }
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int i = 0; i < 16; i += 2) {
+            float e[2];
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              const float x = s[kb][i + y];
+              if constexpr (MASK || ALIBI)
+                e[y] = __builtin_amdgcn_exp2f(x - m_use);
+              else if constexpr (CAP)
+                e[y] = __builtin_amdgcn_exp2f(rule_score(rule, x) - m_use);
+              else
+                e[y] = __builtin_amdgcn_exp2f(fmaf(x, rule.scale, -m_use));
+              l += e[y];
+            }
+            pk[kb][i / 2] = Mat<T>::pack(e[0], e[1]);
+          }
+      };
+      if (full)
+        weights(std::false_type{});
+      else
+        weights(std::true_type{});
+      // O^T += V^T P^T, 16 keys c at a time
+      auto values = [&](int c, int db) {
+        const char* a = vt + voff[db & 3] + (db >> 2) * 256 + 16 * c * RS;
+        const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)a);
+        const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(a + 8 * RS));
+        const u32x2v xx = __builtin_bit_cast(u32x2v, x), yy = __builtin_bit_cast(u32x2v, y);
+        return u32x4v{xx[0], xx[1], yy[0], yy[1]};
+      };
+      if (!careful || full) {
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int c = 0; c < KT / 16; ++c) {
+          const uint32_t* q = &pk[c >> 1][4 * (c & 1)];
+          const u32x4v pt = {q[0], q[1], q[2], q[3]};
+#pragma unroll
+          for (int db = 0; db < DB; ++db) acc[db] = Mat<T>::mma32(values(c, db), pt, acc[db]);
+        }
+        __builtin_amdgcn_s_setprio(0);
+      } else if constexpr (careful) {
+#pragma unroll
+        for (int c = 0; c < KT / 16; ++c) {
+          const uint32_t* q = &pk[c >> 1][4 * (c & 1)];
+          const u32x4v pt = {q[0], q[1], q[2], q[3]};
+#pragma unroll
+          for (int db = 0; db < DB; ++db) {
+            const u32x4v v = values(c, db);
+            u32x4v bad;
+#pragma unroll
+            for (int y = 0; y < 4; ++y) bad[y] = not_finite_halves<Mat<T>::kExp>(v[y]);
+            acc[db] = Mat<T>::mma32(v & ~bad, pt, acc[db]);
+            if (!__any(bad[0] | bad[1] | bad[2] | bad[3])) continue;
+            for (int x = 0; x < 16; ++x) {  // k-element x & 7 of half x >> 3 alone
+              const int j = x & 7, key = k0 + 16 * c + 4 * (x >> 3) + (j & 3) + 8 * (j >> 2);
+              const bool seen = (key >= lo && key < hi) || (key >= lo2 && key < hi2);
+              u32x4v only;
+#pragma unroll
+              for (int y = 0; y < 4; ++y)
+                only[y] = half == (x >> 3) && (j >> 1) == y ? (j & 1 ? 0xffff0000u : 0x0000ffffu) : 0u;
+              const f32x16v one = Mat<T>::mma32(v & bad & only, pt & only, f32x16v{});
+#pragma unroll
+              for (int i = 0; i < 16; ++i) acc[db][i] = seen ? acc[db][i] + one[i] : acc[db][i];
+            }
+          }
+        }
+      }
+    }
+  };
+  run(std::false_type{});
+  float z = l * 0.0f;
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) z = fmaf(acc[db][i], 0.0f, z);
+  if (__syncthreads_or(live && z != z)) run(std::true_type{});
+
+  if (unit >= blocks * g || row >= T_all || !(live || p.zero_rest)) return;
+  l += __shfl_xor(l, 32, 64);
+  const float inv = live ? 1.0f / l : 0.0f;
+  T* dst = (T*)p.out + (int64_t)row * p.out_stride_t + hq * p.out_stride_h + 4 * half;
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      const int d = 32 * db + 8 * (i / 4);
+      if (d < D) {
+        const u32x2v y = {Mat<T>::pack(acc[db][i] * inv, acc[db][i + 1] * inv), Mat<T>::pack(acc[db][i + 2] * inv, acc[db][i + 3] * inv)};
+        *(u32x2v*)(dst + d) = live ? y : u32x2v{0, 0};
+      }
+    }
+}
+
+template <typename T, int DT>
+void launch_packed(const smaq_packed_params& p, const ScoreRule& rule, unsigned grid, int blocks, hipStream_t st) {
+  if (p.score_cap > 0.0f) {
+    if (p.alibi_slopes)
+      packed_kernel<T, DT, true, true><<<grid, kThreads, 0, st>>>(p, rule, blocks);
+    else
+      packed_kernel<T, DT, true, false><<<grid, kThreads, 0, st>>>(p, rule, blocks);
+  } else if (p.alibi_slopes) {
+    packed_kernel<T, DT, false, true><<<grid, kThreads, 0, st>>>(p, rule, blocks);
+  } else {
+    packed_kernel<T, DT, false, false><<<grid, kThreads, 0, st>>>(p, rule, blocks);
+  }
+}
+
 template <typename T>
-__global__ __launch_bounds__(64 * kWaves) void packed_any_kernel(smaq_packed_params p, ScoreRule rule) {
-  const int lane = threadIdx.x & 63;
-  const int64_t row = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
-  if (row >= p.n_tokens * p.n_q_heads) return;
-  const int64_t t = row / p.n_q_heads;
-  const int hq = (int)(row - t * p.n_q_heads), h = hq / (p.n_q_heads / p.n_kv_heads), D = p.head_dim;
-  T* out = (T*)p.out + t * p.out_stride_t + hq * p.out_stride_h;
-  int lo = 0, hi = p.n_docs;  // the document of token t: the last that starts at or before it
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (p.starts[mid] <= t) lo = mid; else hi = mid;
-  }
-  const int64_t s0 = p.n_docs ? max(p.starts[lo], 0) : 0, s1 = p.n_docs ? min((int64_t)p.starts[lo + 1], p.n_tokens) : 0;
-  if (t < s0 || t >= s1) {
-    if (p.zero_rest)
-      for (int d = lane; d < D; d += 64) out[d] = Num<T>::from_f(0.0f);
-    return;
-  }
-  const int64_t i = t - s0, n = s1 - s0;
-  const int64_t prefix = p.prefix_lens ? p.prefix_lens[lo] : 0;
-  const float slope = p.alibi_slopes ? p.alibi_slopes[hq] * kLog2eF : 0.0f;
-  const T* q = (const T*)p.q + t * p.q_stride_t + hq * p.q_stride_h;
-  const T* k = (const T*)p.k + s0 * p.k_stride_t + h * p.k_stride_h;
-  const T* v = (const T*)p.v + s0 * p.v_stride_t + h * p.v_stride_h;
-  float m = -__builtin_inff(), l = 0.0f, o[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int64_t j0 = 0; j0 < n; j0 += 64) {
-    const int64_t j = j0 + lane;
-    const bool seen = j < n && (!p.causal || j <= i || j < prefix) && (!p.window || j > i - p.window || j < prefix);
-    float x = -__builtin_inff();
-    if (seen) {
-      float dot = 0.0f;
-      for (int d = 0; d < D; ++d) dot = fmaf(Num<T>::to_f(q[d]), Num<T>::to_f(k[j * p.k_stride_t + d]), dot);
-      x = rule_score(rule, dot) - slope * (float)llabs(i - j);
-    }
-    const float m_new = fmaxf(m, warp_max(x));
-    const float m_use = m_new == -__builtin_inff() ? 0.0f : m_new;
-    const float w = seen ? exp2f(x - m_use) : 0.0f, a = exp2f(m - m_use);
-    l = l * a + warp_sum(w);
-    m = m_new;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] *= a;
-    const unsigned long long any = __ballot(seen);
-    for (int e = 0; e < 64; ++e) {
-      if (!((any >> e) & 1)) continue;
-      const float we = __shfl(w, e, 64);
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-        if (lane + 64 * c < D) o[c] = fmaf(we, Num<T>::to_f(v[(j0 + e) * p.v_stride_t + lane + 64 * c]), o[c]);
-    }
-  }
-#pragma unroll
-  for (int c = 0; c < 4; ++c)
-    if (lane + 64 * c < D) out[lane + 64 * c] = Num<T>::from_f(o[c] / l);
+void launch_packed(const smaq_packed_params& p, const ScoreRule& rule, unsigned grid, int blocks, hipStream_t st) {
+  if (p.head_dim <= 64)
+    launch_packed<T, 64>(p, rule, grid, blocks, st);
+  else if (p.head_dim <= 128)
+    launch_packed<T, 128>(p, rule, grid, blocks, st);
+  else
+    launch_packed<T, 256>(p, rule, grid, blocks, st);
 }
 
 }  // namespace
@@ -87,12 +403,14 @@ extern "C" int smaq_packed_attention(const smaq_packed_params* p, void* stream) 
   SMAQ_REQUIRE(rows_on_16(p->q, p->q_stride_t, p->q_stride_h) && rows_on_16(p->k, p->k_stride_t, p->k_stride_h) &&
                    rows_on_16(p->v, p->v_stride_t, p->v_stride_h) && rows_on_16(p->out, p->out_stride_t, p->out_stride_h),
                "smaq_packed_attention: rows must start on 16 bytes");
-  const ScoreRule rule = score_rule(p->scale, p->score_cap);
-  const int64_t rows = p->n_tokens * p->n_q_heads;
-  const unsigned blocks = (unsigned)((rows + kWaves - 1) / kWaves);
+  const ScoreRule rule = score_rule(fabsf(p->scale), p->score_cap);  // the kernel gives the sign to the queries
+  const int blocks = (int)((p->n_tokens + 31) / 32), g = p->n_q_heads / p->n_kv_heads;
+  const int64_t grid = ((int64_t)blocks * g + 3) / 4 * p->n_kv_heads;
+  SMAQ_REQUIRE((int64_t)blocks * g < 0x7ffffff0ll && grid <= 0x7fffffffll,
+               "smaq_packed_attention: %lld workgroups are more than one launch takes", (long long)grid);
   if (p->dtype == SMAQ_F16)
-    packed_any_kernel<_Float16><<<blocks, 64 * kWaves, 0, (hipStream_t)stream>>>(*p, rule);
+    launch_packed<_Float16>(*p, rule, (unsigned)grid, blocks, (hipStream_t)stream);
   else
-    packed_any_kernel<bf16><<<blocks, 64 * kWaves, 0, (hipStream_t)stream>>>(*p, rule);
+    launch_packed<bf16>(*p, rule, (unsigned)grid, blocks, (hipStream_t)stream);
   return launch_status("smaq_packed_attention");
 }
