@@ -648,37 +648,55 @@ def attn_hybrid_noalloc(p: AttnParams, device: torch.device) -> None:
 
 # ------------------------------------------------------------- exact path ---
 
-def require_plain(what: str, *tensors) -> None:
-    """The exact path's operators have no derivative: tensors that ask for one
-    are refused."""
-    dual = torch.autograd.forward_ad._current_level >= 0
+def require_inputs(what: str, *tensors) -> int:
+    """The GPU's index that all tensors (None: absent) live on.  The exact path's
+    operators have no derivative: tensors that ask for one are refused."""
+    index, grad = -2, torch.is_grad_enabled()
     for t in tensors:
-        if t is None:
-            continue
-        if (t.requires_grad and torch.is_grad_enabled()) or (
-                dual and torch.autograd.forward_ad.unpack_dual(t).tangent is not None):
-            raise ValueError(f"{what} computes no gradients: call it under torch.no_grad() or detach its inputs")
+        if t is not None:
+            i = t.get_device()
+            if i != index:
+                if index != -2 or i < 0:
+                    require_gpu(*tensors)
+                index = i
+            if grad and t.requires_grad:
+                raise ValueError(f"{what} computes no gradients: call it under torch.no_grad() or detach its inputs")
+    if torch.autograd.forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+                raise ValueError(f"{what} computes no gradients: it takes no dual tensors")
+    return index
 
 
-def launch_on(dev: torch.device, fn, what: str, *args) -> None:
-    """fn(*args, stream) on the device's current stream, with that device current."""
-    if torch.cuda.current_device() == dev.index:
-        _check(fn(*args, _stream(dev)), what)
-        return
-    with torch.cuda.device(dev):
-        _check(fn(*args, _stream(dev)), what)
+def launch_on(index: int, fn, what: str, *args) -> None:
+    """fn(*args, stream) on the current stream of GPU ``index``, with that GPU current."""
+    if torch._C._cuda_getDevice() == index:
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status:
+        _check(status, what)
 
 
-def rows_aligned(t: torch.Tensor, lead: int) -> bool:
-    """Whether the last dim is dense and every row of 16-bit elements starts on
-    16 bytes (the first ``lead`` dims' strides are multiples of 8)."""
-    return (t.stride(-1) == 1 and t.data_ptr() % 16 == 0
-            and all(st % 8 == 0 or n == 1 for n, st in zip(t.shape[:lead], t.stride()[:lead])))
-
-
-def strides(t: torch.Tensor, lead: int) -> list:
-    """The first ``lead`` strides, 0 where a dim has one entry."""
-    return [0 if n == 1 else st for n, st in zip(t.shape[:lead], t.stride()[:lead])]
+def row_steps(t: torch.Tensor):
+    """The strides of 16-bit rows ahead of their dense last dim (0 where a dim has
+    one entry), or None when the last dim is not dense or a row does not start on
+    16 bytes."""
+    *lead, last = t.stride()
+    if last != 1:
+        return None
+    units = t.data_ptr() >> 1
+    for st in lead:
+        units |= st
+    if units & 7:
+        lead = [0 if n == 1 else st for n, st in zip(t.shape, lead)]
+        units = t.data_ptr() >> 1
+        for st in lead:
+            units |= st
+        if units & 7:
+            return None
+    return lead
 
 
 def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:

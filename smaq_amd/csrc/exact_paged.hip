@@ -304,39 +304,63 @@ __global__ __launch_bounds__(kThreads, DT == 256 ? 2 : 3) void paged_kernel(smaq
   }
 }
 
-// The splits of one row joined in their order: one workgroup a row, thread (x, y) dims
-// 4 x of every y-th split.
+// The splits of one row joined in their order: a workgroup a row.  First the splits'
+// weights into LDS, then thread (x, y) sums dims 4 x of every ny-th split, and the ny
+// sums are added in order.
+constexpr int kMaxSplits = 3072;
+
 template <typename T>
 __global__ __launch_bounds__(kThreads) void paged_merge_kernel(smaq_paged_params p, PagedPart part) {
-  __shared__ float so[kThreads][4], sl[kThreads];
-  const int b = blockIdx.x / p.n_q_heads, hq = blockIdx.x % p.n_q_heads, D = p.head_dim;
-  const int nx = D / 4, ny = kThreads / nx, x = threadIdx.x % nx, y = threadIdx.x / nx;
+  __shared__ float sa[kMaxSplits];
+  __shared__ float so[kThreads][4], red[kThreads / 64];
+  const int tid = threadIdx.x, b = blockIdx.x / p.n_q_heads, hq = blockIdx.x % p.n_q_heads, D = p.head_dim;
   int first, last;
   visible(p, b, first, last);
   const int64_t span = last - (first & ~15);
   const int live = last > first ? (int)((span + part.split_len - 1) / part.split_len) : 0;
   const int64_t i0 = (int64_t)blockIdx.x * part.splits;
   float m = kNegInf;
-  for (int s = 0; s < live; ++s) m = fmaxf(m, part.m[i0 + s]);
+  for (int s = tid; s < live; s += kThreads) {
+    sa[s] = part.m[i0 + s];
+    m = fmaxf(m, sa[s]);
+  }
+  m = warp_max(m);
+  if ((tid & 63) == 0) red[tid >> 6] = m;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kThreads / 64; ++w) m = fmaxf(m, red[w]);
+  __syncthreads();
+  // a split of scores of -inf alone (m = -inf, l = NaN) counts only when all are
+  float l = 0.0f;
+  for (int s = tid; s < live; s += kThreads) {
+    const float ms = sa[s];
+    const float a = m == kNegInf ? 1.0f : (ms == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(ms - m));
+    sa[s] = a;
+    if (a != 0.0f) l = fmaf(a, part.l[i0 + s], l);  // NaN is not 0
+  }
+  l = warp_sum(l);
+  if ((tid & 63) == 0) red[tid >> 6] = l;
+  __syncthreads();
+  l = 0.0f;
+#pragma unroll
+  for (int w = 0; w < kThreads / 64; ++w) l += red[w];
+  const int nx = D / 4, ny = kThreads / nx, x = tid % nx, y = tid / nx;
   f32x4v o = {0.f, 0.f, 0.f, 0.f};
-  float sum = 0.0f;
-  if (y < ny)
+  if (y < ny) {
+    const float* src = part.o + i0 * D + 4 * x;
+#pragma unroll 8
     for (int s = y; s < live; s += ny) {
-      const float ms = part.m[i0 + s];
-      if (ms == kNegInf && m != kNegInf) continue;
-      const float a = m == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(ms - m);
-      sum = fmaf(a, part.l[i0 + s], sum);
-      o += a * *(const f32x4v*)(part.o + (i0 + s) * D + 4 * x);
+      const float a = sa[s];
+      const f32x4v v = *(const f32x4v*)(src + (int64_t)s * D);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = a != 0.0f ? fmaf(a, v[e], o[e]) : o[e];
     }
-  *(f32x4v*)so[threadIdx.x] = o;
-  sl[threadIdx.x] = sum;
+  }
+  *(f32x4v*)so[tid] = o;
   __syncthreads();
   if (y != 0) return;
-  for (int k = 1; k < ny; ++k) {
-    sum += sl[x + k * nx];
-    o += *(const f32x4v*)so[x + k * nx];
-  }
-  const float inv = live > 0 && !(m == kNegInf && sum == 0.0f) ? 1.0f / sum : 0.0f;
+  for (int k = 1; k < ny; ++k) o += *(const f32x4v*)so[x + k * nx];
+  const float inv = live > 0 && !(m == kNegInf && l == 0.0f) ? 1.0f / l : 0.0f;
   T* dst = (T*)p.out + (int64_t)b * p.out_stride_b + hq * p.out_stride_h + 4 * x;
   *(u32x2v*)dst = u32x2v{Mat<T>::pack(o[0] * inv, o[1] * inv), Mat<T>::pack(o[2] * inv, o[3] * inv)};
 }
@@ -370,7 +394,7 @@ PagedPart plan_splits(const smaq_paged_params* p) {
   span = std::max<int64_t>(span, 1);
   const int rows = p->n_q_heads / p->n_kv_heads;
   const int64_t units = (int64_t)p->batch * p->n_kv_heads * ((rows + 15) / 16);
-  const int64_t want = 4 * 3 * 256;
+  const int64_t want = kMaxSplits;
   int64_t len = (span * units + want - 1) / want;
   len = std::max<int64_t>((len + kRound - 1) / kRound * kRound, 256);
   PagedPart part{nullptr, nullptr, nullptr, (int)((span + len - 1) / len), len};

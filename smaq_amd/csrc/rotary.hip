@@ -13,7 +13,7 @@
 // goes to sincospif.
 #include <algorithm>
 
-#include "smaq_common.h"
+#include "exact_attention.h"
 
 namespace smaq {
 namespace {
@@ -62,7 +62,7 @@ __device__ __forceinline__ void angle(const RotaryArgs& a, int64_t p, int i, flo
   s *= a.gain;
 }
 
-// One wave per (token, head), one element at a time: every layout and alignment.
+// One wave per (token, head), one element at a time: every head_dim, layout and alignment.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void norm_rotary_any_kernel(RotaryArgs a) {
   const int lane = threadIdx.x & 63;
@@ -101,8 +101,152 @@ __global__ __launch_bounds__(kThreads) void norm_rotary_any_kernel(RotaryArgs a)
   for (int i = a.r + lane; i < a.D; i += 64) out[i] = Num<T>::from_f(normed(i));
 }
 
+// 16 bytes a load: a lane holds two units of E elements, the two halves of E pairs (half
+// layout: units at l E and r/2 + l E; interleaved: neighbours; behind the rotated dims:
+// neighbours), so the rotation needs no exchange and the norm one sum over the
+// `lanes` of a row.  A workgroup takes `tb` tokens: their sines and cosines are formed
+// once into LDS and kept in registers over the heads (queries', then keys'), which
+// `slots` rows of lanes per token take in turn; the first kBatch rows are on their way
+// before the sines are begun.
+constexpr int kBatch = 4;
+
+template <typename T, bool IL>
+__global__ __launch_bounds__(kThreads) void norm_rotary_kernel(RotaryArgs a, int lanes, int tb) {
+  constexpr int E = 16 / (int)sizeof(T);
+  extern __shared__ __attribute__((aligned(16))) float lds[];
+  const int tid = threadIdx.x, half = a.r / 2;
+  float* sw = lds;            // [2][D] weights of queries and keys, offset added
+  float* cs = lds + 2 * a.D;  // [tb][2][r/2]
+  const int64_t t0 = (int64_t)blockIdx.x * tb;
+  const int l = tid & (lanes - 1), row = tid / lanes, slots = kThreads / lanes / tb;
+  const int tok = row / slots, slot = row % slots + blockIdx.y * slots, step = slots * gridDim.y;
+  const int64_t t = t0 + tok;
+  const int nr = a.r / (2 * E), hq = a.in[0].heads, heads = hq + a.in[1].heads;
+  const bool turned = l < nr, live = t < a.tokens && 2 * E * l < a.D;
+  const int ia = IL || !turned ? 2 * E * l : E * l, ib = IL || !turned ? ia + E : half + E * l;
+  const T* xq = (const T*)a.in[0].x + t * a.in[0].st;
+  const T* xk = (const T*)a.in[1].x + t * a.in[1].st;
+  uint4 raw[kBatch][2];
+  auto load = [&](int h0) {
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const int h = h0 + u * step;
+      raw[u][0] = raw[u][1] = uint4{0, 0, 0, 0};
+      if (live && h < heads) {
+        const T* x = h < hq ? xq + h * a.in[0].sh : xk + (h - hq) * a.in[1].sh;
+        raw[u][0] = *(const uint4*)(x + ia);
+        raw[u][1] = *(const uint4*)(x + ib);
+      }
+    }
+  };
+  load(slot);
+#pragma unroll
+  for (int side = 0; side < 2; ++side)
+    if (a.in[side].w)
+      for (int i = tid; i < a.D; i += kThreads) sw[side * a.D + i] = weight_at(a, a.in[side].w, i);
+  for (int i = tid; i < tb * half; i += kThreads) {
+    const int tt = i / half, pair = i - tt * half;
+    if (t0 + tt < a.tokens) angle(a, position(a, t0 + tt), pair, cs[2 * tt * half + pair], cs[(2 * tt + 1) * half + pair]);
+  }
+  const float inv_d = 1.0f / (float)a.D;
+  __syncthreads();
+  float c[E], s[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    c[e] = turned ? cs[2 * tok * half + E * l + e] : 1.0f;
+    s[e] = turned ? cs[(2 * tok + 1) * half + E * l + e] : 0.0f;
+  }
+  for (int h0 = slot; h0 < heads; h0 += kBatch * step) {
+    if (h0 != slot) load(h0);
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const int h = h0 + u * step;
+      if (h >= heads) break;
+      const int side = h < hq ? 0 : 1;
+      float v[2][E];
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        const T* r = (const T*)&raw[u][y];
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[y][e] = Num<T>::to_f(r[e]);
+      }
+      if (side ? a.in[1].w != nullptr : a.in[0].w != nullptr) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+#pragma unroll
+          for (int e = 0; e < E; ++e) sum = fmaf(v[y][e], v[y][e], sum);
+        for (int o = 1; o < lanes; o <<= 1) sum += __shfl_xor(sum, o, 64);
+        const float mean = fmaf(sum, inv_d, a.eps);
+        // the instruction's one ulp; it does not take numbers below the normal range
+        const float inv = mean > 1e-30f ? __builtin_amdgcn_rsqf(mean) : 1.0f / sqrtf(mean);
+        const float* w = sw + side * a.D;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          v[0][e] = v[0][e] * inv * (live ? w[ia + e] : 0.0f);
+          v[1][e] = v[1][e] * inv * (live ? w[ib + e] : 0.0f);
+        }
+      }
+      if (!live) continue;
+      float o[2][E];
+      if constexpr (IL) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const float p = ((const float*)v)[2 * e], q = ((const float*)v)[2 * e + 1];
+          ((float*)o)[2 * e] = turned ? fmaf(p, c[e], -(q * s[e])) : p;
+          ((float*)o)[2 * e + 1] = turned ? fmaf(p, s[e], q * c[e]) : q;
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const float p = v[0][e], q = v[1][e];
+          o[0][e] = turned ? fmaf(p, c[e], -(q * s[e])) : p;
+          o[1][e] = turned ? fmaf(p, s[e], q * c[e]) : q;
+        }
+      }
+      uint4 res[2];
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        uint32_t* r = (uint32_t*)&res[y];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if constexpr (sizeof(T) == 4) r[e] = __float_as_uint(o[y][e]);
+          else r[e] = Mat<T>::pack(o[y][2 * e], o[y][2 * e + 1]);
+        }
+      }
+      T* out = side ? (T*)a.in[1].out + (t * a.in[1].heads + h - hq) * a.D : (T*)a.in[0].out + (t * hq + h) * a.D;
+      *(uint4*)(out + ia) = res[0];
+      *(uint4*)(out + ib) = res[1];
+    }
+  }
+}
+
 template <typename T>
 int launch_rotary(const RotaryArgs& a, hipStream_t st) {
+  constexpr int E = 16 / (int)sizeof(T);
+  bool wide = a.D % (2 * E) == 0 && a.r % (2 * E) == 0 && a.D <= 64 * 2 * E;
+  for (const RotaryIn& in : a.in)
+    wide = wide && (!in.heads || ((uintptr_t)in.x % 16 == 0 && (uintptr_t)in.out % 16 == 0 && in.st % E == 0 && in.sh % E == 0));
+  if (wide) {
+    const int heads = a.in[0].heads + a.in[1].heads;
+    int lanes = 1;
+    while (lanes * 2 * E < a.D) lanes *= 2;
+    // four tokens a workgroup while that leaves four workgroups to a CU; for few tokens the
+    // heads of a token are spread over workgroups as well
+    int tb = 4;
+    while (tb > 1 && (lanes * tb > kThreads || (a.tokens + tb - 1) / tb < 1024)) tb /= 2;
+    const int slots = kThreads / lanes / tb;
+    const int64_t gx = (a.tokens + tb - 1) / tb;
+    const int gy = (int)std::max<int64_t>(1, std::min<int64_t>((heads + slots - 1) / slots, 1024 / gx));
+    SMAQ_REQUIRE(gx <= 0x7fffffffll, "smaq_norm_rotary: %lld tokens are more than one launch takes", (long long)a.tokens);
+    const size_t lds = ((size_t)tb * a.r + 2 * a.D) * sizeof(float);
+    const dim3 grid((unsigned)gx, (unsigned)gy);
+    if (a.interleaved)
+      norm_rotary_kernel<T, true><<<grid, kThreads, lds, st>>>(a, lanes, tb);
+    else
+      norm_rotary_kernel<T, false><<<grid, kThreads, lds, st>>>(a, lanes, tb);
+    return launch_status("smaq_norm_rotary");
+  }
   const int64_t rows = a.tokens * (a.in[0].heads + a.in[1].heads);
   const int64_t blocks = (rows + kThreads / 64 - 1) / (kThreads / 64);
   SMAQ_REQUIRE(blocks <= 0x7fffffffll, "smaq_norm_rotary: %lld rows are more than one launch takes", (long long)rows);

@@ -18,6 +18,9 @@ import torch
 
 from smaq_amd import _native
 
+_INTEGERS = (torch.int32, torch.int64)
+_TYPES = {torch.float16: _native.F16, torch.bfloat16: _native.BF16}
+
 
 def _scores(what: str, head_dim: int, scale: Optional[float], score_cap: float, window: int):
     scale = 1.0 / math.sqrt(head_dim) if scale is None else float(scale)
@@ -33,14 +36,30 @@ def _scores(what: str, head_dim: int, scale: Optional[float], score_cap: float, 
 def _slopes(what: str, alibi_slopes: Optional[torch.Tensor], heads: int):
     if alibi_slopes is None:
         return None
-    if tuple(alibi_slopes.shape) != (heads,) or not alibi_slopes.dtype.is_floating_point:
+    if alibi_slopes.dim() != 1 or alibi_slopes.shape[0] != heads or not alibi_slopes.dtype.is_floating_point:
         raise ValueError(f"{what}: alibi_slopes must be [{heads}] floating point, got {tuple(alibi_slopes.shape)} "
                          f"{alibi_slopes.dtype}")
-    return alibi_slopes.to(torch.float32).contiguous()
+    return (alibi_slopes if alibi_slopes.dtype == torch.float32 else alibi_slopes.float()).contiguous()
+
+
+def _ints(what: str, name: str, t: torch.Tensor, n: int) -> torch.Tensor:
+    """t [n] of integers as contiguous int32."""
+    if t.dim() != 1 or t.shape[0] != n or t.dtype not in _INTEGERS:
+        raise ValueError(f"{what}: {name} must be int32 or int64 [{n}], got {tuple(t.shape)} {t.dtype}")
+    return (t if t.dtype == torch.int32 else t.to(torch.int32)).contiguous()
+
+
+def _rows(t: torch.Tensor):
+    """(t, its row strides), t copied where its rows are not dense or not on 16 bytes."""
+    steps = _native.row_steps(t)
+    if steps is None:
+        t = t.clone(memory_format=torch.contiguous_format)
+        steps = _native.row_steps(t)
+    return t, steps
 
 
 def _heads(what: str, q: torch.Tensor, hkv: int, D: int) -> None:
-    if q.dtype not in (torch.float16, torch.bfloat16):
+    if q.dtype not in _TYPES:
         raise ValueError(f"{what}: float16 or bfloat16 queries, keys and values, got {q.dtype}")
     if D % 8 or not 0 < D <= 256:
         raise ValueError(f"{what}: head_dim must be a multiple of 8 up to 256, got {D}")
@@ -50,7 +69,7 @@ def _heads(what: str, q: torch.Tensor, hkv: int, D: int) -> None:
 
 def _out(what: str, out: Optional[torch.Tensor], q: torch.Tensor, *others: torch.Tensor) -> torch.Tensor:
     if out is None:
-        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        return torch.empty_like(q, memory_format=torch.contiguous_format)
     if (out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous()
             or out.data_ptr() % 16):
         raise ValueError(f"{what}: out must be a contiguous, 16-byte aligned {tuple(q.shape)} {q.dtype} tensor on "
@@ -81,42 +100,31 @@ def compute_packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, 
     result, and left as they are in ``out``.
     """
     what = "compute_packed_attention"
-    dev = _native.require_gpu(q, k, v, cu_seqlens, prefix_lens, alibi_slopes, out)
-    _native.require_plain(what, q, k, v, alibi_slopes, out)
+    index = _native.require_inputs(what, q, k, v, cu_seqlens, prefix_lens, alibi_slopes, out)
     if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]:
         raise ValueError(f"{what}: queries [T, Hq, D] and keys and values [T, Hkv, D] expected, got {tuple(q.shape)}, "
                          f"{tuple(k.shape)}, {tuple(v.shape)}")
     if k.dtype != q.dtype or v.dtype != q.dtype:
         raise ValueError(f"{what}: one dtype for queries, keys and values, got {q.dtype}, {k.dtype}, {v.dtype}")
     T, Hq, D = q.shape
-    _heads(what, q, k.shape[1], D)
+    Hkv = k.shape[1]
+    _heads(what, q, Hkv, D)
     scale, cap, window = _scores(what, D, scale, score_cap, window)
-    if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1 or cu_seqlens.dtype not in (torch.int32, torch.int64):
-        raise ValueError(f"{what}: cu_seqlens must be int32 or int64 [documents + 1], got {tuple(cu_seqlens.shape)} "
-                         f"{cu_seqlens.dtype}")
     docs = cu_seqlens.numel() - 1
-    starts = cu_seqlens.to(torch.int32).contiguous()
-    if prefix_lens is not None:
-        if tuple(prefix_lens.shape) != (docs,) or prefix_lens.dtype not in (torch.int32, torch.int64):
-            raise ValueError(f"{what}: prefix_lens must be int32 or int64 [{docs}], got {tuple(prefix_lens.shape)} "
-                             f"{prefix_lens.dtype}")
-        prefix_lens = prefix_lens.to(torch.int32).contiguous()
+    if docs < 0:
+        raise ValueError(f"{what}: cu_seqlens must be int32 or int64 [documents + 1], got none")
+    starts = _ints(what, "cu_seqlens", cu_seqlens, docs + 1)
+    prefix = None if prefix_lens is None else _ints(what, "prefix_lens", prefix_lens, docs)
     slopes = _slopes(what, alibi_slopes, Hq)
     res = _out(what, out, q, k, v)
-    q, k, v = (t if _native.rows_aligned(t, 2) else t.clone(memory_format=torch.contiguous_format) for t in (q, k, v))
-    p = _native.PackedParams()
-    p.dtype, p.n_docs, p.n_tokens = _native.dtype_code(q.dtype), docs, T
-    p.n_q_heads, p.n_kv_heads, p.head_dim = Hq, k.shape[1], D
-    p.causal, p.window, p.zero_rest, p.scale, p.score_cap = int(bool(causal)), window, int(out is None), scale, cap
-    p.starts = starts.data_ptr()
-    p.prefix_lens = None if prefix_lens is None else prefix_lens.data_ptr()
-    p.alibi_slopes = None if slopes is None else slopes.data_ptr()
-    p.q, p.k, p.v, p.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), res.data_ptr()
-    p.q_stride_t, p.q_stride_h = _native.strides(q, 2)
-    p.k_stride_t, p.k_stride_h = _native.strides(k, 2)
-    p.v_stride_t, p.v_stride_h = _native.strides(v, 2)
-    p.out_stride_t, p.out_stride_h = _native.strides(res, 2)
-    _native.launch_on(dev, _native.lib().smaq_packed_attention, "smaq_packed_attention", ctypes.byref(p))
+    q, (qt, qh) = _rows(q)
+    k, (kt, kh) = _rows(k)
+    v, (vt, vh) = _rows(v)
+    p = _native.PackedParams(
+        _TYPES[q.dtype], docs, Hq, Hkv, D, bool(causal), window, out is None, T, scale, cap, starts.data_ptr(),
+        None if prefix is None else prefix.data_ptr(), None if slopes is None else slopes.data_ptr(), q.data_ptr(),
+        k.data_ptr(), v.data_ptr(), res.data_ptr(), qt, qh, kt, kh, vt, vh, Hq * D, D)
+    _native.launch_on(index, _native.lib().smaq_packed_attention, "smaq_packed_attention", ctypes.byref(p))
     return res
 
 
@@ -140,50 +148,44 @@ def compute_paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     16, cache rows on 16 bytes.
     """
     what = "compute_paged_attention"
-    dev = _native.require_gpu(q, k_cache, v_cache, block_table, seq_lens, alibi_slopes, out)
-    _native.require_plain(what, q, k_cache, v_cache, alibi_slopes, out)
+    index = _native.require_inputs(what, q, k_cache, v_cache, block_table, seq_lens, alibi_slopes, out)
     if q.dim() != 3 or k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.shape[3] != q.shape[2]:
         raise ValueError(f"{what}: queries [B, Hq, D] and caches [blocks, block_size, Hkv, D] expected, got "
                          f"{tuple(q.shape)}, {tuple(k_cache.shape)}, {tuple(v_cache.shape)}")
     if k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
         raise ValueError(f"{what}: one dtype for queries and caches, got {q.dtype}, {k_cache.dtype}, {v_cache.dtype}")
     B, Hq, D = q.shape
-    blocks, bs, hkv, _ = k_cache.shape
-    _heads(what, q, hkv, D)
+    blocks, bs, Hkv, _ = k_cache.shape
+    _heads(what, q, Hkv, D)
     scale, cap, window = _scores(what, D, scale, score_cap, window)
     if bs <= 0 or bs % 16:
         raise ValueError(f"{what}: block_size must be a multiple of 16, got {bs}")
-    if not (_native.rows_aligned(k_cache, 3) and _native.rows_aligned(v_cache, 3)):
+    k_steps, v_steps = _native.row_steps(k_cache), _native.row_steps(v_cache)
+    if k_steps is None or v_steps is None:
         raise ValueError(f"{what}: cache rows must be dense and start on 16 bytes")
-    if block_table.dim() != 2 or block_table.shape[0] < B or block_table.dtype not in (torch.int32, torch.int64):
+    if block_table.dim() != 2 or block_table.shape[0] < B or block_table.dtype not in _INTEGERS:
         raise ValueError(f"{what}: block_table must be an integer [>= {B}, max_blocks] tensor, got "
                          f"{tuple(block_table.shape)} {block_table.dtype}")
-    if seq_lens.dim() != 1 or seq_lens.shape[0] < B or seq_lens.dtype not in (torch.int32, torch.int64):
+    if seq_lens.dim() != 1 or seq_lens.shape[0] < B or seq_lens.dtype not in _INTEGERS:
         raise ValueError(f"{what}: seq_lens must be int32 or int64 [>= {B}], got {tuple(seq_lens.shape)} "
                          f"{seq_lens.dtype}")
     if max_seq_len < 0:
         raise ValueError(f"{what}: max_seq_len must be 0 or more, got {max_seq_len}")
     slopes = _slopes(what, alibi_slopes, Hq)
     res = _out(what, out, q, k_cache, v_cache)
-    if not _native.rows_aligned(q, 2):
-        q = q.clone(memory_format=torch.contiguous_format)
-    table, lens = block_table[:B].to(torch.int32).contiguous(), seq_lens[:B].contiguous()
-    p = _native.PagedParams()
-    p.dtype, p.batch, p.n_q_heads, p.n_kv_heads, p.head_dim = _native.dtype_code(q.dtype), B, Hq, hkv, D
-    p.block_size, p.num_blocks, p.max_blocks, p.window = bs, blocks, table.shape[1], window
-    p.seq_lens_wide, p.max_seq_len, p.scale, p.score_cap = int(lens.dtype == torch.int64), int(max_seq_len), scale, cap
-    p.seq_lens, p.block_table = lens.data_ptr(), table.data_ptr()
-    p.alibi_slopes = None if slopes is None else slopes.data_ptr()
-    p.q, p.k_cache, p.v_cache, p.out = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), res.data_ptr()
-    p.q_stride_b, p.q_stride_h = _native.strides(q, 2)
-    p.out_stride_b, p.out_stride_h = _native.strides(res, 2)
-    p.k_stride_block, p.k_stride_t, p.k_stride_h = _native.strides(k_cache, 3)
-    p.v_stride_block, p.v_stride_t, p.v_stride_h = _native.strides(v_cache, 3)
-    lib = _native.lib()
-    size = lib.smaq_paged_workspace_bytes(ctypes.byref(p))
-    if size < 0:
-        _native._check(-1, "smaq_paged_attention")
-    ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
-    p.workspace, p.workspace_bytes = (None if ws is None else ws.data_ptr()), size
-    _native.launch_on(dev, lib.smaq_paged_attention, "smaq_paged_attention", ctypes.byref(p))
+    q, (qb, qh) = _rows(q)
+    table = (block_table if block_table.dtype == torch.int32 else block_table.to(torch.int32)).contiguous()
+    lens = seq_lens.contiguous()
+    p = _native.PagedParams(
+        _TYPES[q.dtype], B, Hq, Hkv, D, bs, blocks, table.shape[1], window, lens.dtype == torch.int64, int(max_seq_len),
+        scale, cap, lens.data_ptr(), table.data_ptr(), None if slopes is None else slopes.data_ptr(), q.data_ptr(),
+        k_cache.data_ptr(), v_cache.data_ptr(), res.data_ptr(), qb, qh, Hq * D, D, *k_steps, *v_steps)
+    lib, ref = _native.lib(), ctypes.byref(p)
+    size = lib.smaq_paged_workspace_bytes(ref)
+    if size:
+        if size < 0:
+            _native._check(-1, "smaq_paged_attention")
+        ws = torch.empty(size, dtype=torch.uint8, device=q.device)
+        p.workspace, p.workspace_bytes = ws.data_ptr(), size
+    _native.launch_on(index, lib.smaq_paged_attention, "smaq_paged_attention", ref)
     return res

@@ -7,12 +7,14 @@ both from the requests' lengths without reading one back to the host.
 
 from __future__ import annotations
 
-import ctypes
 from typing import NamedTuple
 
 import torch
 
 from smaq_amd import _native
+
+
+_LENGTHS = (torch.int32, torch.int64)
 
 
 class PageStep(NamedTuple):
@@ -39,14 +41,11 @@ def build_page_step(context_lens: torch.Tensor, new_lens: torch.Tensor, block_ta
     counted in ``status[1]``; ``status[0]`` is the number of pages the step takes
     off the list, more than it holds when it was too short.
     """
-    dev = _native.require_gpu(context_lens, new_lens, block_table, free_blocks)
+    index = _native.require_inputs("build_page_step", context_lens, new_lens, block_table, free_blocks)
+    n = context_lens.shape[0] if context_lens.dim() else -1
     for t, what in ((context_lens, "context_lens"), (new_lens, "new_lens")):
-        if t.dim() != 1 or t.dtype not in (torch.int32, torch.int64):
-            raise ValueError(f"build_page_step: {what} must be a one-dimensional int32 or int64 tensor, got "
-                             f"{tuple(t.shape)} {t.dtype}")
-    n = context_lens.shape[0]
-    if new_lens.shape[0] != n:
-        raise ValueError(f"build_page_step: {new_lens.shape[0]} new lengths for {n} requests")
+        if t.dim() != 1 or t.shape[0] != n or t.dtype not in _LENGTHS:
+            raise ValueError(f"build_page_step: {what} must be int32 or int64 [requests], got {tuple(t.shape)} {t.dtype}")
     if (block_table.dim() != 2 or block_table.shape[0] < n or block_table.dtype != torch.int32
             or not block_table.is_contiguous()):
         raise ValueError(f"build_page_step: block_table must be a contiguous int32 [>= {n}, max_blocks] tensor, got "
@@ -54,20 +53,24 @@ def build_page_step(context_lens: torch.Tensor, new_lens: torch.Tensor, block_ta
     if free_blocks.dim() != 1 or free_blocks.dtype != torch.int32:
         raise ValueError(f"build_page_step: free_blocks must be a one-dimensional int32 tensor, got "
                          f"{tuple(free_blocks.shape)} {free_blocks.dtype}")
-    for t, what in ((context_lens, "context_lens"), (new_lens, "new_lens"), (free_blocks, "free_blocks")):
-        if _native.overlap(block_table, t):
-            raise ValueError(f"build_page_step: block_table shares memory with {what}")
     ctx, new, free = context_lens.contiguous(), new_lens.contiguous(), free_blocks.contiguous()
+    table, width = block_table.data_ptr(), block_table.shape[1]
+    end = table + 4 * block_table.shape[0] * width
+    for t, what in ((ctx, "context_lens"), (new, "new_lens"), (free, "free_blocks")):
+        start = t.data_ptr()
+        if start < end and start + t.shape[0] * t.element_size() > table:
+            raise ValueError(f"build_page_step: block_table shares memory with {what}")
     num_tokens = int(num_tokens)
     if num_tokens < 0:
         raise ValueError(f"build_page_step: num_tokens must be 0 or more, got {num_tokens}")
-    step = PageStep(torch.empty(num_tokens, dtype=torch.int64, device=dev),
-                    torch.empty(num_tokens, dtype=torch.int64, device=dev),
-                    torch.empty(n + 1, dtype=torch.int32, device=dev), torch.empty(n, dtype=torch.int32, device=dev),
-                    torch.empty(2, dtype=torch.int32, device=dev))
-    ptr = ctypes.c_void_p
-    _native.launch_on(dev, _native.lib().smaq_page_step, "smaq_page_step", ptr(ctx.data_ptr()), ctx.element_size(),
-                      ptr(new.data_ptr()), new.element_size(), n, ptr(block_table.data_ptr()), block_table.shape[1],
-                      ptr(free.data_ptr()), free.shape[0], int(block_size), num_tokens,
-                      *(ptr(t.data_ptr()) for t in step))
-    return step
+    dev = block_table.device
+    slots = torch.empty(num_tokens, dtype=torch.int64, device=dev)
+    positions = torch.empty(num_tokens, dtype=torch.int64, device=dev)
+    starts = torch.empty(n + 1, dtype=torch.int32, device=dev)
+    seq_lens = torch.empty(n, dtype=torch.int32, device=dev)
+    status = torch.empty(2, dtype=torch.int32, device=dev)
+    _native.launch_on(index, _native.lib().smaq_page_step, "smaq_page_step", ctx.data_ptr(), ctx.element_size(),
+                      new.data_ptr(), new.element_size(), n, table, width, free.data_ptr(), free.shape[0],
+                      int(block_size), num_tokens, slots.data_ptr(), positions.data_ptr(), starts.data_ptr(),
+                      seq_lens.data_ptr(), status.data_ptr())
+    return PageStep(slots, positions, starts, seq_lens, status)

@@ -98,15 +98,15 @@ class RotaryPositions:
         return new
 
 
-def _side(what: str, x: Optional[torch.Tensor], like: torch.Tensor):
+def _heads(what: str, x: torch.Tensor, lead, D: int, dtype) -> torch.Tensor:
     """x [*lead, H, D] as [T, H, D] (a view where its strides allow)."""
-    if x is None:
-        return None
-    if x.dim() < 2 or x.shape[:-2] != like.shape[:-2] or x.shape[-1] != like.shape[-1] or x.dtype != like.dtype:
-        raise ValueError(f"apply_norm_rotary: {what} {tuple(x.shape)} {x.dtype} does not match queries "
-                         f"{tuple(like.shape)} {like.dtype} in tokens, head_dim or dtype")
-    flat = x.reshape(math.prod(x.shape[:-2]), *x.shape[-2:])
-    return flat if flat.stride(-1) == 1 or flat.shape[-1] == 1 else flat.contiguous()
+    shape = x.shape
+    if len(shape) < 2 or shape[:-2] != lead or shape[-1] != D or x.dtype != dtype:
+        raise ValueError(f"apply_norm_rotary: {what} {tuple(x.shape)} {x.dtype} do not match queries of tokens "
+                         f"{tuple(lead)}, head_dim {D} and {dtype}")
+    if len(shape) != 3:
+        x = x.reshape(math.prod(lead), *shape[-2:])
+    return x if x.stride(2) == 1 or D == 1 else x.contiguous()
 
 
 def apply_norm_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, rotary: RotaryPositions,
@@ -121,35 +121,45 @@ def apply_norm_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: tor
     rounding.  Views of a packed projection are read in place; the results are
     new contiguous tensors, (q, k), or (q, None).
     """
-    dev = _native.require_gpu(q, k, positions, rotary.freqs, q_weight, k_weight)
-    _native.require_plain("apply_norm_rotary", q, k, q_weight, k_weight)
+    freqs = rotary.freqs
+    index = _native.require_inputs("apply_norm_rotary", q, k, positions, freqs, q_weight, k_weight)
     if q.dim() < 2:
         raise ValueError(f"apply_norm_rotary: queries must be [*lead, heads, head_dim], got {tuple(q.shape)}")
-    if tuple(positions.shape) != tuple(q.shape[:-2]) or positions.dtype not in (torch.int32, torch.int64):
-        raise ValueError(f"apply_norm_rotary: positions must be int32 or int64 {tuple(q.shape[:-2])}, got "
+    shape, dtype = q.shape, q.dtype
+    lead, D = shape[:-2], shape[-1]
+    wide = positions.dtype == torch.int64
+    if positions.shape != lead or not (wide or positions.dtype == torch.int32):
+        raise ValueError(f"apply_norm_rotary: positions must be int32 or int64 {tuple(lead)}, got "
                          f"{tuple(positions.shape)} {positions.dtype}")
-    D = q.shape[-1]
-    weights = [w for w in (q_weight, k_weight) if w is not None]
-    for w in weights:
-        if tuple(w.shape) != (D,) or w.dtype != weights[0].dtype:
-            raise ValueError(f"apply_norm_rotary: weights must be [{D}] and of one dtype, got {tuple(w.shape)} {w.dtype}")
-    if not (eps >= 0.0 and math.isfinite(eps) and math.isfinite(weight_offset)):
+    weight_dtype = None
+    for w in (q_weight, k_weight):
+        if w is not None:
+            weight_dtype = weight_dtype or w.dtype
+            if w.dim() != 1 or w.shape[0] != D or w.dtype != weight_dtype:
+                raise ValueError(f"apply_norm_rotary: weights must be [{D}] and of one dtype, got {tuple(w.shape)} "
+                                 f"{w.dtype}")
+    if not (0.0 <= eps < math.inf and math.isfinite(weight_offset)):
         raise ValueError("apply_norm_rotary: eps must be a finite number of 0 or more, weight_offset finite")
-    code = _native.dtype_code(q.dtype)
-    qf, kf, pos = _side("queries", q, q), _side("keys", k, q), positions.reshape(-1).contiguous()
-    qw, kw = (None if w is None else w.contiguous() for w in (q_weight, k_weight))
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    k_out = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=dev)
-    p = _native.RotaryParams()
-    p.dtype, p.n_q_heads, p.head_dim, p.tokens = code, qf.shape[1], D, qf.shape[0]
-    p.q, p.q_stride_t, p.q_stride_h, p.q_out = qf.data_ptr(), qf.stride(0), qf.stride(1), q_out.data_ptr()
-    if kf is not None:
-        p.n_k_heads, p.k, p.k_out = kf.shape[1], kf.data_ptr(), k_out.data_ptr()
-        p.k_stride_t, p.k_stride_h = kf.stride(0), kf.stride(1)
-    p.rotary_dim, p.interleaved, p.gain = rotary.rotary_dim, int(rotary.interleaved), rotary.gain
-    p.freqs, p.positions, p.position_bytes = rotary.freqs.data_ptr(), pos.data_ptr(), pos.element_size()
-    p.q_weight, p.k_weight = (None if w is None else w.data_ptr() for w in (qw, kw))
-    p.weight_dtype = _native.dtype_code(weights[0].dtype) if weights else _native.F32
-    p.eps, p.weight_offset = eps, weight_offset
-    _native.launch_on(dev, _native.lib().smaq_norm_rotary, "smaq_norm_rotary", ctypes.byref(p))
+    code = _native.dtype_code(dtype)
+    weight_code = _native.F32 if weight_dtype is None else _native.dtype_code(weight_dtype)
+    qf = _heads("queries", q, lead, D, dtype)
+    pos = positions.reshape(-1) if len(lead) != 1 else positions
+    pos = pos.contiguous()
+    qw = q_weight if q_weight is None else q_weight.contiguous()
+    kw = k_weight if k_weight is None else k_weight.contiguous()
+    q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    k_out = None
+    T, Hq, _ = qf.shape
+    Hk = kp = ko = kst = ksh = 0
+    if k is not None:
+        kf = _heads("keys", k, lead, D, dtype)
+        k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
+        Hk, kp, ko = kf.shape[1], kf.data_ptr(), k_out.data_ptr()
+        kst, ksh, _ = kf.stride()
+    qst, qsh, _ = qf.stride()
+    p = _native.RotaryParams(
+        code, Hq, Hk, D, rotary.rotary_dim, rotary.interleaved, T, qf.data_ptr(), qst, qsh, kp, kst, ksh,
+        q_out.data_ptr(), ko, pos.data_ptr(), 8 if wide else 4, freqs.data_ptr(), rotary.gain,
+        None if qw is None else qw.data_ptr(), None if kw is None else kw.data_ptr(), weight_code, eps, weight_offset)
+    _native.launch_on(index, _native.lib().smaq_norm_rotary, "smaq_norm_rotary", ctypes.byref(p))
     return q_out, k_out

@@ -88,7 +88,9 @@ def test_cpu_tensors_are_refused():
 @pytest.fixture
 def no_gpu_check(monkeypatch):
     """The checks of arguments behind the device check, on CPU tensors; no call gets as far as a launch."""
+    check = _native.require_inputs
     monkeypatch.setattr(_native, "require_gpu", lambda *t: torch.device("cuda", 0))
+    monkeypatch.setattr(_native, "require_inputs", lambda *a: (check(*a), 0)[1])
 
     def launch(*a, **k):
         raise AssertionError("launched")
