@@ -34,15 +34,30 @@ inline ScoreRule score_rule(float scale, float cap) {
 
 // cap tanh(x / cap) of x = scale dot, times log2(e).  The limits at +-inf are exact,
 // NaN passes.
-__device__ __forceinline__ float rule_score(const ScoreRule& r, float dot) {
+template <bool WIDE>
+__device__ __forceinline__ float capped_score(const ScoreRule& r, float dot) {
   const float x = dot * r.scale;
-  if (r.cap == 0.0f) return x;
   const float t = fmaf(-2.0f * r.cap, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x) + 1.0f), r.cap);
-  if (!r.wide) return t;
+  if constexpr (!WIDE) return t;
   // y = x / (2 log2 e): y - y^3/3 + 2 y^5/15 - 17 y^7/315 + 62 y^9/2835, below 0.35 to 2^-21
   const float y = x * (0.5f / kLog2eF), z = y * y;
   const float s = fmaf(z, fmaf(z, fmaf(z, 62.0f / 2835.0f, -17.0f / 315.0f), 2.0f / 15.0f), -1.0f / 3.0f);
   return fabsf(y) < 0.35f ? r.cap * fmaf(y * z, s, y) : t;
+}
+
+// put(i, score of the product get(i)) for N products: one uniform choice of the rule
+template <int N, typename Get, typename Put>
+__device__ __forceinline__ void each_score(const ScoreRule& r, Get get, Put put) {
+  if (r.cap == 0.0f) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) put(i, get(i) * r.scale);
+  } else if (!r.wide) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) put(i, capped_score<false>(r, get(i)));
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) put(i, capped_score<true>(r, get(i)));
+  }
 }
 
 // ------------------------------------------------------- matrix operands ---

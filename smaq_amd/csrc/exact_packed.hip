@@ -73,7 +73,7 @@ __device__ __forceinline__ int wave_max(int v) {
   return __builtin_amdgcn_readfirstlane(v);
 }
 
-template <typename T, int DT, bool CAP, bool ALIBI>
+template <typename T, int DT, bool FULL, bool CAP, bool ALIBI>
 __global__ __launch_bounds__(kThreads, 2) void packed_kernel(smaq_packed_params p, ScoreRule rule, int blocks) {
   constexpr int KT = DT == 256 ? 32 : 64;  // keys per tile
   constexpr int KB = KT / 32;              // 32-key blocks
@@ -141,33 +141,49 @@ __global__ __launch_bounds__(kThreads, 2) void packed_kernel(smaq_packed_params 
     gap1 = min(gap1, __builtin_amdgcn_readfirstlane(span[x][3]));
   }
 
-  // ---- queries: column n, dims 16 ks + 8 half ..; a negative scale is taken into them
+  // ---- queries: column n, dims 16 ks + 8 half ..; a negative scale is taken into them,
+  // and a scale of 0 makes them 0
   u32x4v qr[KS];
   {
     const T* src = (const T*)p.q + (int64_t)row * p.q_stride_t + hq * p.q_stride_h;
-    const uint32_t flip = p.scale < 0.0f ? 0x80008000u : 0u;
+    const uint32_t flip = p.scale < 0.0f ? 0x80008000u : 0u, keep = p.scale == 0.0f ? 0u : ~0u;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       qr[ks] = u32x4v{0, 0, 0, 0};
-      if (live && 16 * ks + 8 * half < D) qr[ks] = *(const u32x4v*)(src + 16 * ks + 8 * half) ^ flip;
+      if (live && (FULL || 16 * ks + 8 * half < D)) qr[ks] = (*(const u32x4v*)(src + 16 * ks + 8 * half) ^ flip) & keep;
     }
   }
   const float slope = ALIBI ? (live ? p.alibi_slopes[hq] * kLog2eF : 0.0f) : 0.0f;
 
-  // ---- tile copies: load i of thread tid fills unit 256 i + tid of the tile
+  // ---- tile copies: load i of thread tid fills unit 256 i + tid of the tile, of row
+  // i kThreads / UPR + tid / UPR
+  constexpr int RPL = kThreads / UPR;  // rows of a load
   const T* kc = (const T*)p.k + h * p.k_stride_h;
   const T* vc = (const T*)p.v + h * p.v_stride_h;
+  const int r0 = tid / UPR, u0 = tid % UPR;
+  auto to_lds = [&](const void* src, char* dst) {
+    __builtin_amdgcn_global_load_lds(src, (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
+  };
   auto copy_tile = [&](int k, int buf) {
-    char* kd = lds + buf * 2 * TILE;
+    char* kd = lds + buf * 2 * TILE + 1024 * w;
+    if (FULL && k + KT <= k_hi) {
+      // whole tiles: a base of the wave and a 32-bit offset of the lane
+      const uint32_t ko = (uint32_t)(2 * r0 * (int)p.k_stride_t), vo = (uint32_t)(2 * r0 * (int)p.v_stride_t);
 #pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        const int r = i * RPL + r0;
+        to_lds((const char*)(kc + (int64_t)(k + i * RPL) * p.k_stride_t) + (ko + 16 * (u0 ^ key_swizzle<DT>(r))), kd + 4096 * i);
+        to_lds((const char*)(vc + (int64_t)(k + i * RPL) * p.v_stride_t) + (vo + 16 * (u0 ^ val_swizzle<DT>(r))), kd + TILE + 4096 * i);
+      }
+      return;
+    }
+#pragma unroll 1
     for (int i = 0; i < LOADS; ++i) {
-      const int r = (kThreads * i + tid) / UPR, u = tid % UPR;
+      const int r = i * RPL + r0;
       const int64_t key = min(k + r, k_hi - 1);
-      const int uk = u ^ key_swizzle<DT>(r), uv = u ^ val_swizzle<DT>(r);
-      const void* ks = 8 * uk < D ? (const void*)(kc + key * p.k_stride_t + 8 * uk) : (const void*)&kZeroUnit;
-      const void* vs = 8 * uv < D ? (const void*)(vc + key * p.v_stride_t + 8 * uv) : (const void*)&kZeroUnit;
-      __builtin_amdgcn_global_load_lds(ks, (__attribute__((address_space(3))) void*)(kd + 16 * (kThreads * i + 64 * w)), 16, 0, 0);
-      __builtin_amdgcn_global_load_lds(vs, (__attribute__((address_space(3))) void*)(kd + TILE + 16 * (kThreads * i + 64 * w)), 16, 0, 0);
+      const int uk = u0 ^ key_swizzle<DT>(r), uv = u0 ^ val_swizzle<DT>(r);
+      to_lds(FULL || 8 * uk < D ? (const void*)(kc + key * p.k_stride_t + 8 * uk) : (const void*)&kZeroUnit, kd + 4096 * i);
+      to_lds(FULL || 8 * uv < D ? (const void*)(vc + key * p.v_stride_t + 8 * uv) : (const void*)&kZeroUnit, kd + TILE + 4096 * i);
     }
   };
   // the tile behind k: the next keys, or past the gap
@@ -176,16 +192,11 @@ __global__ __launch_bounds__(kThreads, 2) void packed_kernel(smaq_packed_params 
     return k >= gap0 && k + KT <= gap1 && gap1 < k_hi ? gap1 : k;
   };
 
-  // ---- operand addresses within a tile
-  const int krow = n * RS;
-  int koff[KS];
-#pragma unroll
-  for (int ks = 0; ks < KS; ++ks) koff[ks] = krow + 16 * ((2 * ks + half) ^ key_swizzle<DT>(n));
+  // ---- operand addresses within a tile: rows are multiples of RS, so a step along the
+  // units of a row is an XOR of the whole address
+  const int koff = n * RS + 16 * (half ^ key_swizzle<DT>(n));
   const int vr0 = 4 * half + ((lane & 15) >> 2);
-  int voff[DB < 4 ? DB : 4];
-#pragma unroll
-  for (int db = 0; db < (DB < 4 ? DB : 4); ++db)
-    voff[db] = vr0 * RS + 16 * ((4 * db + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) ^ val_swizzle<DT>(vr0)) + 8 * (lane & 1);
+  const int voff = vr0 * RS + 16 * ((2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) ^ val_swizzle<DT>(vr0)) + 8 * (lane & 1);
 
   f32x16v acc[DB];
   float m_ref, m_use, m_thr, l;
@@ -210,8 +221,7 @@ __global__ __launch_bounds__(kThreads, 2) void packed_kernel(smaq_packed_params 
       const int k0 = k;
       k = k_next;
       if (k0 >= w_hi || k0 + KT <= w_lo || (k0 >= w_gap0 && k0 + KT <= w_gap1)) continue;
-      const char* kt = lds + buf * 2 * TILE;
-      const char* vt = kt + TILE;
+      const int kt = buf * 2 * TILE + koff, vt = buf * 2 * TILE + TILE + voff;
       f32x16v s[KB];
       __builtin_amdgcn_s_setprio(1);
 #pragma unroll
@@ -219,74 +229,88 @@ __global__ __launch_bounds__(kThreads, 2) void packed_kernel(smaq_packed_params 
         s[kb] = f32x16v{};
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks)
-          s[kb] = Mat<T>::mma32(*(const u32x4v*)(kt + koff[ks] + kb * 32 * RS), qr[ks], s[kb]);
+          s[kb] = Mat<T>::mma32(*(const u32x4v*)(lds + (kt ^ (32 * ks)) + kb * 32 * RS), qr[ks], s[kb]);
       }
       __builtin_amdgcn_s_setprio(0);
       // key of register i of block kb: k0 + 32 kb + 8 (i / 4) + 4 half + i % 4
       const bool full = k0 >= w_full0 && k0 + KT <= w_full1;
-      const float gap = ALIBI ? (float)(row - k0 - 4 * half) : 0.0f;
-      uint32_t pk[KB][8];
-      auto weights = [&](auto masked) {
-        constexpr bool MASK = decltype(masked)::value;
-        float mx = kNegInf;
-        if constexpr (MASK || ALIBI) {
+      auto get = [&](int i) { return s[i / 16][i % 16]; };
+      if constexpr (ALIBI) {
+        const float gap = (float)(row - k0 - 4 * half);
+        auto put = [&](int i, float x) {
+          s[i / 16][i % 16] = fmaf(-slope, fabsf(gap - (float)(32 * (i / 16) + 8 * (i % 16 / 4) + i % 4)), x);
+        };
+        if constexpr (CAP) {
+          each_score<16 * KB>(rule, get, put);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16 * KB; ++i) put(i, get(i) * rule.scale);
+        }
+      }
+      if (!full) {
+        const int a0 = lo - k0 - 4 * half, a1 = hi - k0 - 4 * half, b0 = lo2 - k0 - 4 * half, b1 = hi2 - k0 - 4 * half;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int key = 32 * kb + 8 * (i / 4) + i % 4;
+            const bool seen = ((key >= a0) & (key < a1)) | ((key >= b0) & (key < b1));
+            s[kb][i] = seen ? s[kb][i] : kNegInf;
+          }
+      }
+      float mx = kNegInf;
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kb][i]);
+      if constexpr (CAP && !ALIBI)
+        mx = rule.wide ? capped_score<true>(rule, mx) : capped_score<false>(rule, mx);
+      else if constexpr (!ALIBI)
+        mx *= rule.scale;
+      if (__any(mx > m_thr)) {
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        const float m_new = fmaxf(m_ref, mx);
+        m_use = m_new == kNegInf ? 0.0f : m_new;
+        const float alpha = __builtin_amdgcn_exp2f(m_ref - m_use);
+        l *= alpha;
+#pragma unroll
+        for (int db = 0; db < DB; ++db) acc[db] *= alpha;
+        m_ref = m_new;
+        m_thr = m_new + kRaise;
+      }
+      if constexpr (CAP && !ALIBI) {
+        each_score<16 * KB>(rule, get, [&](int i, float x) { s[i / 16][i % 16] = __builtin_amdgcn_exp2f(x - m_use); });
+      } else {
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            s[kb][i] = __builtin_amdgcn_exp2f(ALIBI ? s[kb][i] - m_use : fmaf(s[kb][i], rule.scale, -m_use));
+      }
+      if constexpr (CAP && !ALIBI) {  // the cap brings a masked score back to -cap
+        if (!full) {
+          const int a0 = lo - k0 - 4 * half, a1 = hi - k0 - 4 * half, b0 = lo2 - k0 - 4 * half, b1 = hi2 - k0 - 4 * half;
 #pragma unroll
           for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-              float x = CAP ? rule_score(rule, s[kb][i]) : s[kb][i] * rule.scale;
-              if constexpr (ALIBI) x = fmaf(-slope, fabsf(gap - (float)(32 * kb + 8 * (i / 4) + i % 4)), x);
-              if constexpr (MASK) {
-                const int key = k0 + 4 * half + 32 * kb + 8 * (i / 4) + i % 4;
-                x = (key >= lo && key < hi) || (key >= lo2 && key < hi2) ? x : kNegInf;
-              }
-              s[kb][i] = x;
-              mx = fmaxf(mx, x);
+              const int key = 32 * kb + 8 * (i / 4) + i % 4;
+              const bool seen = ((key >= a0) & (key < a1)) | ((key >= b0) & (key < b1));
+              s[kb][i] = seen ? s[kb][i] : 0.0f;
             }
-        } else {
-#pragma unroll
-          for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kb][i]);
-          mx = CAP ? rule_score(rule, mx) : mx * rule.scale;
         }
-        if (__any(mx > m_thr)) {
-          mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-          const float m_new = fmaxf(m_ref, mx);
-          m_use = m_new == kNegInf ? 0.0f : m_new;
-          const float alpha = __builtin_amdgcn_exp2f(m_ref - m_use);
-          l *= alpha;
+      }
+      uint32_t pk[KB][8];
 #pragma unroll
-          for (int db = 0; db < DB; ++db) acc[db] *= alpha;
-          m_ref = m_new;
-          m_thr = m_new + kRaise;
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+          l += s[kb][i] + s[kb][i + 1];
+          pk[kb][i / 2] = Mat<T>::pack(s[kb][i], s[kb][i + 1]);
         }
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-          for (int i = 0; i < 16; i += 2) {
-            float e[2];
-#pragma unroll
-            for (int y = 0; y < 2; ++y) {
-              const float x = s[kb][i + y];
-              if constexpr (MASK || ALIBI)
-                e[y] = __builtin_amdgcn_exp2f(x - m_use);
-              else if constexpr (CAP)
-                e[y] = __builtin_amdgcn_exp2f(rule_score(rule, x) - m_use);
-              else
-                e[y] = __builtin_amdgcn_exp2f(fmaf(x, rule.scale, -m_use));
-              l += e[y];
-            }
-            pk[kb][i / 2] = Mat<T>::pack(e[0], e[1]);
-          }
-      };
-      if (full)
-        weights(std::false_type{});
-      else
-        weights(std::true_type{});
       // O^T += V^T P^T, 16 keys c at a time
       auto values = [&](int c, int db) {
-        const char* a = vt + voff[db & 3] + (db >> 2) * 256 + 16 * c * RS;
+        const char* a = lds + (vt ^ (64 * (db & 3))) + (db >> 2) * 256 + 16 * c * RS;
         const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)a);
         const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(a + 8 * RS));
         const u32x2v xx = __builtin_bit_cast(u32x2v, x), yy = __builtin_bit_cast(u32x2v, y);
@@ -348,25 +372,35 @@ __global__ __launch_bounds__(kThreads, 2) void packed_kernel(smaq_packed_params 
 #pragma unroll
     for (int i = 0; i < 16; i += 4) {
       const int d = 32 * db + 8 * (i / 4);
-      if (d < D) {
+      if (FULL || d < D) {
         const u32x2v y = {Mat<T>::pack(acc[db][i] * inv, acc[db][i + 1] * inv), Mat<T>::pack(acc[db][i + 2] * inv, acc[db][i + 3] * inv)};
         *(u32x2v*)(dst + d) = live ? y : u32x2v{0, 0};
       }
     }
 }
 
-template <typename T, int DT>
+template <typename T, int DT, bool FULL>
 void launch_packed(const smaq_packed_params& p, const ScoreRule& rule, unsigned grid, int blocks, hipStream_t st) {
   if (p.score_cap > 0.0f) {
     if (p.alibi_slopes)
-      packed_kernel<T, DT, true, true><<<grid, kThreads, 0, st>>>(p, rule, blocks);
+      packed_kernel<T, DT, FULL, true, true><<<grid, kThreads, 0, st>>>(p, rule, blocks);
     else
-      packed_kernel<T, DT, true, false><<<grid, kThreads, 0, st>>>(p, rule, blocks);
+      packed_kernel<T, DT, FULL, true, false><<<grid, kThreads, 0, st>>>(p, rule, blocks);
   } else if (p.alibi_slopes) {
-    packed_kernel<T, DT, false, true><<<grid, kThreads, 0, st>>>(p, rule, blocks);
+    packed_kernel<T, DT, FULL, false, true><<<grid, kThreads, 0, st>>>(p, rule, blocks);
   } else {
-    packed_kernel<T, DT, false, false><<<grid, kThreads, 0, st>>>(p, rule, blocks);
+    packed_kernel<T, DT, FULL, false, false><<<grid, kThreads, 0, st>>>(p, rule, blocks);
   }
+}
+
+template <typename T, int DT>
+void launch_packed(const smaq_packed_params& p, const ScoreRule& rule, unsigned grid, int blocks, hipStream_t st) {
+  // a whole tile's lane offsets fit 32 bits (else every row is addressed by itself)
+  const bool near = p.k_stride_t >= 0 && p.k_stride_t < (1 << 24) && p.v_stride_t >= 0 && p.v_stride_t < (1 << 24);
+  if (p.head_dim == DT && near)
+    launch_packed<T, DT, true>(p, rule, grid, blocks, st);
+  else
+    launch_packed<T, DT, false>(p, rule, grid, blocks, st);
 }
 
 template <typename T>
@@ -403,7 +437,8 @@ extern "C" int smaq_packed_attention(const smaq_packed_params* p, void* stream) 
   SMAQ_REQUIRE(rows_on_16(p->q, p->q_stride_t, p->q_stride_h) && rows_on_16(p->k, p->k_stride_t, p->k_stride_h) &&
                    rows_on_16(p->v, p->v_stride_t, p->v_stride_h) && rows_on_16(p->out, p->out_stride_t, p->out_stride_h),
                "smaq_packed_attention: rows must start on 16 bytes");
-  const ScoreRule rule = score_rule(fabsf(p->scale), p->score_cap);  // the kernel gives the sign to the queries
+  // the kernel gives the scale's sign, and a scale of 0, to the queries
+  const ScoreRule rule = score_rule(p->scale == 0.0f ? 1.0f : fabsf(p->scale), p->score_cap);
   const int blocks = (int)((p->n_tokens + 31) / 32), g = p->n_q_heads / p->n_kv_heads;
   const int64_t grid = ((int64_t)blocks * g + 3) / 4 * p->n_kv_heads;
   SMAQ_REQUIRE((int64_t)blocks * g < 0x7ffffff0ll && grid <= 0x7fffffffll,

@@ -186,11 +186,11 @@ __global__ __launch_bounds__(kThreads, DT == 256 ? 2 : 3) void paged_kernel(smaq
     const bool whole = id[0] >= 0 && id[1] >= 0 && t >= first && t + 32 <= end;
     float x[2][4], mx = kNegInf;
     const float gap = (float)(last - 1 - t - 4 * g);
+    each_score<8>(rule, [&](int i) { return s[i / 4][i % 4]; }, [&](int i, float y) { x[i / 4][i % 4] = y; });
 #pragma unroll
     for (int a = 0; a < 2; ++a)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        x[a][i] = rule_score(rule, s[a][i]);
         if (p.alibi_slopes) x[a][i] = fmaf(-slope, gap - (float)(16 * a + i), x[a][i]);
         if (!whole) {
           const int tok = t + 16 * a + 4 * g + i;
