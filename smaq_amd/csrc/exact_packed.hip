@@ -95,52 +95,6 @@ __global__ __launch_bounds__(kThreads, 2) void packed_kernel(smaq_packed_params 
   const int tb = unit / g, hq = h * g + unit % g;
   const int row = 32 * tb + n;
 
-  // ---- the ranges of this lane's row: [lo, hi), and [lo2, hi2) if the prefix is apart
-  int lo = 0, hi = 0, lo2 = 0, hi2 = 0;
-  if (unit < blocks * g && p.n_docs > 0) {
-    const int t0 = 32 * tb, t1 = min(t0 + 31, T_all - 1);
-    int d = wave_last(p.starts, p.n_docs, t0, lane);
-    const int d1 = wave_last(p.starts, p.n_docs, t1, lane);
-    for (int end = d1 + 1; end - d > 1;) {
-      const int mid = (d + end) >> 1;
-      if (p.starts[mid] <= row) d = mid; else end = mid;
-    }
-    const int s = max(p.starts[d], 0), e = min(p.starts[d + 1], T_all);
-    if (row >= s && row < e) {
-      lo = p.window ? max(s, row - p.window + 1) : s;
-      hi = p.causal ? row + 1 : e;
-      const int pre = p.prefix_lens ? s + min(max(p.prefix_lens[d], 0), e - s) : s;
-      if (pre >= lo) {
-        lo = s;
-        hi = max(hi, pre);
-      } else if (pre > s) {
-        lo2 = s;
-        hi2 = pre;
-      }
-    }
-  }
-  const bool live = hi > lo;
-  const bool apart = hi2 > lo2;
-  // of the wave: first and last key, the gap no row looks into, the keys all rows see
-  const int w_lo = wave_min(live ? (apart ? lo2 : lo) : kIntMax), w_hi = wave_max(live ? hi : 0);
-  const int w_gap0 = wave_max(apart ? hi2 : (live ? lo : 0)), w_gap1 = wave_min(live ? lo : kIntMax);
-  const int w_full0 = wave_max(live ? lo : 0), w_full1 = wave_min(live ? hi : kIntMax);
-  if (lane == 0) {
-    span[w][0] = w_lo;
-    span[w][1] = w_hi;
-    span[w][2] = w_gap0;
-    span[w][3] = w_gap1;
-  }
-  __syncthreads();
-  int k_lo = kIntMax, k_hi = 0, gap0 = 0, gap1 = kIntMax;
-#pragma unroll
-  for (int x = 0; x < 4; ++x) {
-    k_lo = min(k_lo, __builtin_amdgcn_readfirstlane(span[x][0]));
-    k_hi = max(k_hi, __builtin_amdgcn_readfirstlane(span[x][1]));
-    gap0 = max(gap0, __builtin_amdgcn_readfirstlane(span[x][2]));
-    gap1 = min(gap1, __builtin_amdgcn_readfirstlane(span[x][3]));
-  }
-
   // ---- queries: column n, dims 16 ks + 8 half ..; a negative scale is taken into them,
   // and a scale of 0 makes them 0
   u32x4v qr[KS];
@@ -150,9 +104,97 @@ __global__ __launch_bounds__(kThreads, 2) void packed_kernel(smaq_packed_params 
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       qr[ks] = u32x4v{0, 0, 0, 0};
-      if (live && (FULL || 16 * ks + 8 * half < D)) qr[ks] = (*(const u32x4v*)(src + 16 * ks + 8 * half) ^ flip) & keep;
+      if (row < T_all && unit < blocks * g && (FULL || 16 * ks + 8 * half < D)) qr[ks] = (*(const u32x4v*)(src + 16 * ks + 8 * half) ^ flip) & keep;
     }
   }
+  // ---- the ranges of this lane's row: [lo, hi), and [lo2, hi2) if the prefix is apart;
+  // and of the wave: first and last key, the gap no row looks into, the keys all rows see
+  int lo = 0, hi = 0, lo2 = 0, hi2 = 0;
+  int w_lo = kIntMax, w_hi = 0, w_gap0 = 0, w_gap1 = kIntMax, w_full0 = 0, w_full1 = kIntMax;
+  auto see = [&](int t, int s, int e, int prefix, int& a0, int& a1, int& b0, int& b1) {
+    a0 = p.window ? max(s, t - p.window + 1) : s;
+    a1 = p.causal ? t + 1 : e;
+    b0 = b1 = 0;
+    const int pre = s + min(max(prefix, 0), e - s);
+    if (pre >= a0) {
+      a0 = s;
+      a1 = max(a1, pre);
+    } else if (pre > s) {
+      b0 = s;
+      b1 = pre;
+    }
+  };
+  if (unit < blocks * g && p.n_docs > 0) {
+    const int t0 = 32 * tb, t1 = min(t0 + 31, T_all - 1);
+    int d0, d1, v = 0;
+    const bool few = p.n_docs < 64;  // the starts of all documents in one register
+    if (few) {
+      v = p.starts[min(lane, p.n_docs)];
+      const unsigned long long at0 = __ballot(lane < p.n_docs && v <= t0), at1 = __ballot(lane < p.n_docs && v <= t1);
+      d0 = max((int)__popcll(at0) - 1, 0);
+      d1 = max((int)__popcll(at1) - 1, 0);
+    } else {
+      d0 = wave_last(p.starts, p.n_docs, t0, lane);
+      d1 = wave_last(p.starts, p.n_docs, t1, lane);
+    }
+    if (d0 == d1) {
+      // rows of one document: lo, hi, and whether the prefix is apart do not fall from row
+      // to row, so the first and last row bound the wave
+      const int s = max(few ? __builtin_amdgcn_readlane(v, d0) : p.starts[d0], 0);
+      const int e = min(few ? __builtin_amdgcn_readlane(v, d0 + 1) : p.starts[d0 + 1], T_all);
+      const int prefix = p.prefix_lens ? p.prefix_lens[d0] : 0;
+      const int ra = max(t0, s), rb = min(t1, e - 1);
+      if (ra <= rb) {
+        int x0, x1, a_lo, a_hi, b_lo, b_hi;
+        see(ra, s, e, prefix, a_lo, a_hi, x0, x1);
+        see(rb, s, e, prefix, b_lo, b_hi, x0, x1);
+        const bool rb_apart = x1 > x0;
+        w_lo = rb_apart ? s : a_lo;
+        w_hi = b_hi;
+        w_gap0 = rb_apart ? x1 : b_lo;
+        w_gap1 = a_lo;
+        w_full0 = b_lo;
+        w_full1 = a_hi;
+        if (row >= ra && row <= rb) see(row, s, e, prefix, lo, hi, lo2, hi2);
+      }
+    } else {
+      int d = d0;
+      for (int end = d1 + 1; end - d > 1;) {
+        const int mid = (d + end) >> 1;
+        if (p.starts[mid] <= row) d = mid; else end = mid;
+      }
+      const int s = max(p.starts[d], 0), e = min(p.starts[d + 1], T_all);
+      if (row >= s && row < e) see(row, s, e, p.prefix_lens ? p.prefix_lens[d] : 0, lo, hi, lo2, hi2);
+      const bool in = hi > lo, out = hi2 > lo2;
+      w_lo = wave_min(in ? (out ? lo2 : lo) : kIntMax);
+      w_hi = wave_max(in ? hi : 0);
+      w_gap0 = wave_max(out ? hi2 : (in ? lo : 0));
+      w_gap1 = wave_min(in ? lo : kIntMax);
+      w_full0 = wave_max(in ? lo : 0);
+      w_full1 = wave_min(in ? hi : kIntMax);
+    }
+  }
+  const bool live = hi > lo;
+  const bool w_apart = __any(hi2 > lo2);
+  // of the workgroup; waves of one block have the same (the branch is the workgroup's)
+  int k_lo = w_lo, k_hi = w_hi, gap0 = w_gap0, gap1 = w_gap1;
+  if ((unit - w) / g != (unit - w + 3) / g) {
+    if (lane == 0) {
+      span[w][0] = w_lo;
+      span[w][1] = w_hi;
+      span[w][2] = w_gap0;
+      span[w][3] = w_gap1;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      k_lo = min(k_lo, __builtin_amdgcn_readfirstlane(span[x][0]));
+      k_hi = max(k_hi, __builtin_amdgcn_readfirstlane(span[x][1]));
+      gap0 = max(gap0, __builtin_amdgcn_readfirstlane(span[x][2]));
+      gap1 = min(gap1, __builtin_amdgcn_readfirstlane(span[x][3]));
+    }
+  }
+
   const float slope = ALIBI ? (live ? p.alibi_slopes[hq] * kLog2eF : 0.0f) : 0.0f;
 
   // ---- tile copies: load i of thread tid fills unit 256 i + tid of the tile, of row
@@ -247,7 +289,13 @@ __global__ __launch_bounds__(kThreads, 2) void packed_kernel(smaq_packed_params 
           for (int i = 0; i < 16 * KB; ++i) put(i, get(i) * rule.scale);
         }
       }
-      if (!full) {
+      if (!full && !w_apart && k0 >= w_full0) {  // causal and last tiles: cut above only
+        const int a1 = hi - k0 - 4 * half;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[kb][i] = 32 * kb + 8 * (i / 4) + i % 4 < a1 ? s[kb][i] : kNegInf;
+      } else if (!full) {
         const int a0 = lo - k0 - 4 * half, a1 = hi - k0 - 4 * half, b0 = lo2 - k0 - 4 * half, b1 = hi2 - k0 - 4 * half;
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
