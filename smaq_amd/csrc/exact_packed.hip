@@ -83,6 +83,10 @@ __global__ __launch_bounds__(kThreads, 2) void packed_kernel(smaq_packed_params 
   constexpr int RS = DT * 2;               // bytes of a row
   constexpr int TILE = KT * RS;            // bytes of a key or value tile
   constexpr int LOADS = KT * UPR / kThreads;
+  // Matrix sections at raised wave priority: 16384 capped tokens 2.69 -> 2.64 ms, 256 dims
+  // 1.17 -> 1.12 ms; without a cap at up to 128 dims they are better left alone (2.14 -> 2.11
+  // ms, 8192 tokens of 8 / 8 heads 231 -> 214 us).
+  constexpr bool PRIO = CAP || DT == 256;
   __shared__ __attribute__((aligned(16))) char lds[4 * TILE];  // two buffers of (keys, values)
   __shared__ int span[4][4];
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, half = lane >> 5;
@@ -265,7 +269,7 @@ __global__ __launch_bounds__(kThreads, 2) void packed_kernel(smaq_packed_params 
       if (k0 >= w_hi || k0 + KT <= w_lo || (k0 >= w_gap0 && k0 + KT <= w_gap1)) continue;
       const int kt = buf * 2 * TILE + koff, vt = buf * 2 * TILE + TILE + voff;
       f32x16v s[KB];
-      __builtin_amdgcn_s_setprio(1);
+      if constexpr (PRIO) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) {
         s[kb] = f32x16v{};
@@ -273,7 +277,7 @@ __global__ __launch_bounds__(kThreads, 2) void packed_kernel(smaq_packed_params 
         for (int ks = 0; ks < KS; ++ks)
           s[kb] = Mat<T>::mma32(*(const u32x4v*)(lds + (kt ^ (32 * ks)) + kb * 32 * RS), qr[ks], s[kb]);
       }
-      __builtin_amdgcn_s_setprio(0);
+      if constexpr (PRIO) __builtin_amdgcn_s_setprio(0);
       // key of register i of block kb: k0 + 32 kb + 8 (i / 4) + 4 half + i % 4
       const bool full = k0 >= w_full0 && k0 + KT <= w_full1;
       auto get = [&](int i) { return s[i / 16][i % 16]; };
@@ -365,7 +369,7 @@ __global__ __launch_bounds__(kThreads, 2) void packed_kernel(smaq_packed_params 
         return u32x4v{xx[0], xx[1], yy[0], yy[1]};
       };
       if (!careful || full) {
-        __builtin_amdgcn_s_setprio(1);
+        if constexpr (PRIO) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int c = 0; c < KT / 16; ++c) {
           const uint32_t* q = &pk[c >> 1][4 * (c & 1)];
@@ -373,7 +377,7 @@ __global__ __launch_bounds__(kThreads, 2) void packed_kernel(smaq_packed_params 
 #pragma unroll
           for (int db = 0; db < DB; ++db) acc[db] = Mat<T>::mma32(values(c, db), pt, acc[db]);
         }
-        __builtin_amdgcn_s_setprio(0);
+        if constexpr (PRIO) __builtin_amdgcn_s_setprio(0);
       } else if constexpr (careful) {
 #pragma unroll
         for (int c = 0; c < KT / 16; ++c) {

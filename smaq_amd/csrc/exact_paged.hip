@@ -16,10 +16,16 @@
 //                                 D/16 block with v_perm; matrix e holds dims
 //                                 n D/16 + e.
 //
-// A wave has its own running maximum and sum; four waves take 32-token steps in
-// turn, so a workgroup covers 128 tokens a round.  Keys of the next step are
-// loaded as soon as this step's products have read theirs, values likewise: half
-// of a step's 16 KB is in flight at any time.
+// A wave has its own running maximum and sum.  Keys of the next step are loaded as
+// soon as this step's products have read theirs, values likewise: half of a step's
+// 16 KB is in flight at any time.  The four waves of a workgroup take the steps of one
+// head in turn, or four heads side by side (HW = 4): rows of four heads lie next to each
+// other, and reading them together is kinder to the memory.
+//
+// All steps of the batch are dealt to the workgroups in equal shares, however long
+// each sequence is: a share begins and ends inside sequences, and a row whose steps
+// went to several workgroups is joined from their partial results in order by a second
+// launch.  Nothing is atomic; the result depends on the lengths and the launch alone.
 #include <algorithm>
 
 #include "exact_attention.h"
@@ -28,14 +34,42 @@ namespace smaq {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kRound = 128;  // tokens of a round of the four waves
+constexpr int kMaxShares = 1024;
+constexpr uint32_t kLeastSteps = 2;  // of a share
 constexpr int64_t kLongest = 0x7fff0000;  // positions fit an int, those of 32 rounds ahead too
 
-struct PagedPart {  // partials of [batch * n_q_heads] rows and `splits` splits
-  float *m, *l, *o;
-  int splits;
-  int64_t split_len;
+// How the work is dealt.  `shares` 0: workgroup u takes unit u whole and no merge follows.
+// Else share i holds the steps [i W / shares, (i + 1) W / shares) of all W, in the order
+// sequence, unit, step; a unit that lies in several shares leaves in each a slot of
+// slot_rows rows: slot 1 of the share it starts in, slot 0 of the others.
+struct PagedPlan {
+  int group;      // heads that a workgroup takes side by side
+  int units;      // per sequence: head groups x tiles of 16 query rows
+  int tiles;      // of one head group
+  int slot_rows;  // heads of a group x rows of a tile
+  int shares;
+  float *m, *l, *o;  // [shares][2][slot_rows], o with head_dim
+  uint32_t* base;    // [batch] first step of each sequence; [batch]: W (below 2^31)
 };
+
+// W = `all` steps dealt to the shares that have some (kLeastSteps or more each): the first
+// `more` hold each + 1, the others each.
+struct Deal {
+  uint32_t each, more, shares;
+  __device__ __forceinline__ Deal(uint32_t all, uint32_t most) {
+    shares = max(1u, min(most, all / kLeastSteps));
+    each = all / shares;
+    more = all - each * shares;
+  }
+  __device__ __forceinline__ uint32_t start(uint32_t i) const { return i * each + min(i, more); }
+  __device__ __forceinline__ uint32_t owner(uint32_t step) const {
+    const uint32_t low = more * (each + 1);
+    return step < low ? step / (each + 1) : more + (step - low) / max(each, 1u);
+  }
+};
+
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); }
 
 // the tokens [first, end) that sequence b's query sees
 __device__ __forceinline__ void visible(const smaq_paged_params& p, int b, int& first, int& end) {
@@ -45,322 +79,418 @@ __device__ __forceinline__ void visible(const smaq_paged_params& p, int b, int& 
   first = p.window && end > p.window ? end - p.window : 0;
 }
 
-template <typename T, int DT, bool FULL>
+// steps of `step` tokens of a unit of sequence b; they start on a page's 16 tokens
+__device__ __forceinline__ int unit_steps(const smaq_paged_params& p, int b, int step) {
+  int first, last;
+  visible(p, b, first, last);
+  return last > first ? (int)(((int64_t)last - (first & ~15) + step - 1) / step) : 0;
+}
+
+template <typename T, int DT, bool FULL, int HW, bool WHOLE>
 __global__ __launch_bounds__(kThreads, DT == 256 ? 2 : 3) void paged_kernel(smaq_paged_params p, ScoreRule rule,
-                                                                           PagedPart part) {
-  constexpr int KC = DT / 32;  // k steps of a product over the head dim
-  constexpr int VE = DT / 16;  // dims of a lane, matrices of a V step
-  constexpr int VW = VE / 2;   // words of a lane's value row
+                                                                           PagedPlan plan) {
+  constexpr int KC = DT / 32;   // k steps of a product over the head dim
+  constexpr int VE = DT / 16;   // dims of a lane, matrices of a V step
+  constexpr int VW = VE / 2;    // words of a lane's value row
+  constexpr int WPH = 4 / HW;   // waves of a head
+  constexpr int STEP = 32 * WPH;
   constexpr int OS = DT + 4;
   __shared__ float so[4][16][OS];
   __shared__ float sm[4][16], sl[4][16];
   // at 256 dims the queries stay in LDS: with them in registers the loop spills
   constexpr bool QL = DT == 256;
+  static_assert(!QL || HW == 1, "the waves share the queries in LDS");
   __shared__ uint32_t sq[QL ? 16 : 1][DT / 2 + 4];
-  const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int rows = p.n_q_heads / p.n_kv_heads, tiles = (rows + 15) / 16;
-  int idx = blockIdx.x;
-  const int tile = idx % tiles;
-  idx /= tiles;
-  const int h = idx % p.n_kv_heads;
-  idx /= p.n_kv_heads;
-  const int split = idx % part.splits, b = idx / part.splits;
-  int first, last;
-  visible(p, b, first, last);
-  const int64_t begin64 = (first & ~15) + split * part.split_len;
-  const int begin = (int)min(begin64, (int64_t)last), end = (int)min(begin64 + part.split_len, (int64_t)last);
-  const bool direct = part.splits == 1;
-  if (begin >= end && !direct) return;  // the merge knows
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int rows = p.n_q_heads / p.n_kv_heads, D = p.head_dim, bs = p.block_size;
 
-  const int D = p.head_dim, bs = p.block_size;
-  const int row = 16 * tile + n, hq = h * rows + row;
-  const int* table = p.block_table + (int64_t)b * p.max_blocks;
-  const T* kc = (const T*)p.k_cache + h * p.k_stride_h;
-  const T* vc = (const T*)p.v_cache + h * p.v_stride_h;
-  const uint32_t klane = (uint32_t)(2 * n * p.k_stride_t + 16 * g);
-  const uint32_t vlane = (uint32_t)(2 * 4 * g * p.v_stride_t + 2 * VE * n);
-
-  auto load_q = [&](int c) {
-    u32x4v x = {0, 0, 0, 0};
-    if (row < rows && (FULL || 32 * c + 8 * g < D))
-      x = *(const u32x4v*)((const T*)p.q + (int64_t)b * p.q_stride_b + hq * p.q_stride_h + 32 * c + 8 * g);
-    return x;
-  };
-  u32x4v qr[QL ? 1 : KC];
-  if constexpr (QL) {
-#pragma unroll
-    for (int c = 0; c < KC; c += 4) *(u32x4v*)&sq[n][16 * (c + w) + 4 * g] = load_q(c + w);
-    __syncthreads();
+  // ---- this workgroup's steps [at, at_end) and the sequence b (first step `base`) of the first
+  int b;
+  uint32_t base = 0, at = 0, at_end = 1;
+  if constexpr (WHOLE) {
+    b = blockIdx.x / plan.units;
   } else {
+    // every wave sums the sequences' steps, a run of sequences a lane, and finds the run and
+    // then the sequence that hold its first step
+    auto scan = [&](uint32_t sum) {
 #pragma unroll
-    for (int c = 0; c < KC; ++c) qr[c] = load_q(c);
+      for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t x = __shfl_up(sum, o, 64);
+        sum += lane >= o ? x : 0;
+      }
+      return sum;
+    };
+    const uint32_t units = plan.units;
+    const int run = (p.batch + 63) / 64;
+    uint32_t sum = 0;
+    for (int i = lane * run, e = min(p.batch, i + run); i < e; ++i) sum += unit_steps(p, i, STEP);
+    const uint32_t in = scan(sum);
+    const uint32_t all = (uint32_t)__builtin_amdgcn_readlane((int)in, 63) * units;
+    const Deal deal(all, plan.shares);
+    if (blockIdx.x == 0 && tid == 0) plan.base[p.batch] = all;
+    at_end = 0;
+    if (blockIdx.x < deal.shares) {
+      at = uniform(deal.start(blockIdx.x));
+      at_end = uniform(deal.start(blockIdx.x + 1));
+    }
+    // the lanes whose run ends at or before the first step come first
+    const int in_run = min((int)__popcll(__ballot(in * units <= at)), 63);
+    b = in_run * run;
+    base = (uint32_t)__builtin_amdgcn_readlane((int)(in - sum), in_run) * units;
+    for (int left = run; left > 1 && at < at_end; left -= 64) {
+      const int i = b + lane;
+      const uint32_t mine = lane < left && i < p.batch ? unit_steps(p, i, STEP) : 0;
+      const uint32_t upto = scan(mine);
+      const int past = (int)__popcll(__ballot(base + upto * units <= at));
+      if (past < 64) {
+        base += (uint32_t)__builtin_amdgcn_readlane((int)(upto - mine), past) * units;
+        b += past;
+        break;
+      }
+      base += (uint32_t)__builtin_amdgcn_readlane((int)upto, 63) * units;
+      b += 64;
+    }
+    // rows that see no token
+    for (int i = blockIdx.x; i < p.batch; i += gridDim.x)
+      if (unit_steps(p, i, STEP) == 0)
+        for (int u = tid; u < p.n_q_heads * (D / 4); u += kThreads)
+          *(u32x2v*)((T*)p.out + (int64_t)i * p.out_stride_b + (u / (D / 4)) * p.out_stride_h + 4 * (u % (D / 4))) = u32x2v{0, 0};
+    if (at >= at_end) return;
   }
-  const float slope = p.alibi_slopes && row < rows ? p.alibi_slopes[hq] * kLog2eF : 0.0f;
+  const uint32_t at_first = at;
 
-  // pages of this wave's next 32 steps, two 16-token tiles each, one per lane
-  auto load_ids = [&](int t) {
-    const int tt = t + kRound * (lane >> 1) + 16 * (lane & 1);
-    int id = -1;
-    if (tt < end) id = table[(uint32_t)tt / (uint32_t)bs];
-    return id >= 0 && id < p.num_blocks ? id : -1;
-  };
+  while (at < at_end) {
+    int first, last;
+    visible(p, b, first, last);
+    first = uniform(first);
+    last = uniform(last);
+    int unit, begin = first & ~15, end = last;
+    bool direct = true;
+    uint32_t unit0 = 0, stop = at_end;
+    if constexpr (WHOLE) {
+      unit = blockIdx.x % plan.units;
+    } else {
+      const uint32_t steps = last > first ? (uint32_t)(last - begin + STEP - 1) / STEP : 0, here = steps * plan.units;
+      if (at >= base + here) {
+        base += here;
+        ++b;
+        continue;
+      }
+      if (at == base && tid == 0) plan.base[b] = base;
+      unit = uniform((at - base) / steps);
+      unit0 = base + unit * steps;
+      stop = min(unit0 + steps, at_end);
+      direct = at == unit0 && stop == unit0 + steps;
+      end = min(begin + (int)(stop - unit0) * STEP, last);
+      begin += (int)(at - unit0) * STEP;
+    }
 
-  f32x4v acc[VE];
+    const int tile = unit % plan.tiles, h0 = unit / plan.tiles * HW, h = HW == 1 ? h0 : h0 + w;
+    const int row = 16 * tile + n, hq = h * rows + row;
+    const int* table = p.block_table + (int64_t)b * p.max_blocks;
+    const T* kc = (const T*)p.k_cache + h * p.k_stride_h;
+    const T* vc = (const T*)p.v_cache + h * p.v_stride_h;
+    const uint32_t klane = (uint32_t)(2 * n * p.k_stride_t + 16 * g);
+    const uint32_t vlane = (uint32_t)(2 * 4 * g * p.v_stride_t + 2 * VE * n);
+
+    auto load_q = [&](int c) {
+      u32x4v x = {0, 0, 0, 0};
+      if (row < rows && (FULL || 32 * c + 8 * g < D))
+        x = *(const u32x4v*)((const T*)p.q + (int64_t)b * p.q_stride_b + hq * p.q_stride_h + 32 * c + 8 * g);
+      return x;
+    };
+    u32x4v qr[QL ? 1 : KC];
+    if constexpr (QL) {
 #pragma unroll
-  for (int e = 0; e < VE; ++e) acc[e] = f32x4v{0.f, 0.f, 0.f, 0.f};
-  float m_ref = kNegInf, m_use = 0.0f, m_thr = kNegInf, l = 0.0f;
-  bool some = false;
-
-  u32x4v kr[2][KC];
-  uint32_t vr[2][4][VW];
-  auto load_k = [&](int t, const int* id) {
+      for (int c = 0; c < KC; c += 4) *(u32x4v*)&sq[n][16 * (c + w) + 4 * g] = load_q(c + w);
+      __syncthreads();
+    } else {
 #pragma unroll
-    for (int a = 0; a < 2; ++a) {
-      const uint32_t off = (uint32_t)(t + 16 * a) % (uint32_t)bs;
-      const char* src = (const char*)(kc + (int64_t)max(id[a], 0) * p.k_stride_block + (int64_t)off * p.k_stride_t);
+      for (int c = 0; c < KC; ++c) qr[c] = load_q(c);
+    }
+    const float slope = p.alibi_slopes && row < rows ? p.alibi_slopes[hq] * kLog2eF : 0.0f;
+
+    // pages of this wave's next 32 steps, two 16-token tiles each, one per lane
+    auto load_ids = [&](int t) {
+      const int tt = t + STEP * (lane >> 1) + 16 * (lane & 1);
+      int id = -1;
+      if (tt < end) id = table[(uint32_t)tt / (uint32_t)bs];
+      return id >= 0 && id < p.num_blocks ? id : -1;
+    };
+
+    f32x4v acc[VE];
+#pragma unroll
+    for (int e = 0; e < VE; ++e) acc[e] = f32x4v{0.f, 0.f, 0.f, 0.f};
+    float m_ref = kNegInf, m_use = 0.0f, m_thr = kNegInf, l = 0.0f;
+    bool some = false;
+
+    u32x4v kr[2][KC];
+    uint32_t vr[2][4][VW];
+    auto load_k = [&](int t, const int* id) {
+#pragma unroll
+      for (int a = 0; a < 2; ++a) {
+        const uint32_t off = (uint32_t)(t + 16 * a) % (uint32_t)bs;
+        const char* src = (const char*)(kc + (int64_t)max(id[a], 0) * p.k_stride_block + (int64_t)off * p.k_stride_t);
+#pragma unroll
+        for (int c = 0; c < KC; ++c) {
+          if (FULL || 32 * c + 8 * g < D)
+            kr[a][c] = *(const u32x4v*)(src + klane + 64 * c);
+          else
+            kr[a][c] = u32x4v{0, 0, 0, 0};
+        }
+      }
+    };
+    // whether the rows of a step are all there and seen
+    auto whole_step = [&](int t, const int* id) { return id[0] >= 0 && id[1] >= 0 && t >= first && t + 32 <= end; };
+    // a value that is not seen must not meet its zero weight: it is read as 0
+    auto load_v = [&](int t, const int* id) {
+      const bool inside = whole_step(t, id);
+#pragma unroll
+      for (int a = 0; a < 2; ++a) {
+        const uint32_t off = (uint32_t)(t + 16 * a) % (uint32_t)bs;
+        const char* src = (const char*)(vc + (int64_t)max(id[a], 0) * p.v_stride_block + (int64_t)off * p.v_stride_t);
+        auto rows_of = [&](auto seen) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const char* r = src + 2 * j * p.v_stride_t + vlane;
+            if constexpr (VW == 2) {
+              u32x2v x = {0, 0};
+              if (seen(j) && (FULL || VE * n < D)) x = *(const u32x2v*)r;
+              vr[a][j][0] = x[0];
+              vr[a][j][1] = x[1];
+            } else {
+#pragma unroll
+              for (int c = 0; c < VW / 4; ++c) {
+                u32x4v x = {0, 0, 0, 0};
+                if (seen(j) && (FULL || VE * n + 8 * c < D)) x = *(const u32x4v*)(r + 16 * c);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) vr[a][j][4 * c + e] = x[e];
+              }
+            }
+          }
+        };
+        if (inside)
+          rows_of([](int) { return true; });
+        else
+          rows_of([&](int j) {
+            const int tok = t + 16 * a + 4 * g + j;
+            return id[a] >= 0 && tok >= first && tok < end;
+          });
+      }
+    };
+
+    int t = begin + 32 * (w % WPH);
+    int step = 0, ids = -1, id[2], nid[2];
+    if (t < end) {
+      ids = load_ids(t);
+      id[0] = __builtin_amdgcn_readlane(ids, 0);
+      id[1] = __builtin_amdgcn_readlane(ids, 1);
+      load_k(t, id);
+      load_v(t, id);
+    }
+    for (; t < end; t += STEP) {
+      const bool more = t + STEP < end;
+      if (more) {
+        if (++step == 32) {
+          step = 0;
+          ids = load_ids(t + STEP);
+        }
+        nid[0] = __builtin_amdgcn_readlane(ids, 2 * step);
+        nid[1] = __builtin_amdgcn_readlane(ids, 2 * step + 1);
+      }
+      f32x4v s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+      if constexpr (QL) asm volatile("" ::: "memory");  // read again each step
 #pragma unroll
       for (int c = 0; c < KC; ++c) {
-        if (FULL || 32 * c + 8 * g < D)
-          kr[a][c] = *(const u32x4v*)(src + klane + 64 * c);
-        else
-          kr[a][c] = u32x4v{0, 0, 0, 0};
+        u32x4v q;
+        if constexpr (QL) q = *(const u32x4v*)&sq[n][16 * c + 4 * g]; else q = qr[c];
+#pragma unroll
+        for (int a = 0; a < 2; ++a) s[a] = Mat<T>::mma16(kr[a][c], q, s[a]);
       }
-    }
-  };
-  auto load_v = [&](int t, const int* id) {
+      if (more) load_k(t + STEP, nid);
+      const bool inside = whole_step(t, id);
+      float x[2][4], mx = kNegInf;
+      const float gap = (float)(last - 1 - t - 4 * g);
+      each_score<8>(rule, [&](int i) { return s[i / 4][i % 4]; }, [&](int i, float y) { x[i / 4][i % 4] = y; });
 #pragma unroll
-    for (int a = 0; a < 2; ++a) {
-      const uint32_t off = (uint32_t)(t + 16 * a) % (uint32_t)bs;
-      const char* src = (const char*)(vc + (int64_t)max(id[a], 0) * p.v_stride_block + (int64_t)off * p.v_stride_t);
+      for (int a = 0; a < 2; ++a)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const char* r = src + 2 * j * p.v_stride_t + vlane;
-        if constexpr (VW == 2) {
-          u32x2v x = {0, 0};
-          if (FULL || VE * n < D) x = *(const u32x2v*)r;
-          vr[a][j][0] = x[0];
-          vr[a][j][1] = x[1];
-        } else {
-#pragma unroll
-          for (int c = 0; c < VW / 4; ++c) {
-            u32x4v x = {0, 0, 0, 0};
-            if (FULL || VE * n + 8 * c < D) x = *(const u32x4v*)(r + 16 * c);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) vr[a][j][4 * c + e] = x[e];
+        for (int i = 0; i < 4; ++i) {
+          if (p.alibi_slopes) x[a][i] = fmaf(-slope, gap - (float)(16 * a + i), x[a][i]);
+          if (!inside) {
+            const int tok = t + 16 * a + 4 * g + i;
+            const bool ok = id[a] >= 0 && tok >= first && tok < end;
+            x[a][i] = ok ? x[a][i] : kNegInf;
+            some |= ok;
           }
+          mx = fmaxf(mx, x[a][i]);
         }
+      some |= inside;
+      if (__any(mx > m_thr)) {
+        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        const float m_new = fmaxf(m_ref, mx);
+        m_use = m_new == kNegInf ? 0.0f : m_new;
+        const float alpha = __builtin_amdgcn_exp2f(m_ref - m_use);
+        l *= alpha;
+#pragma unroll
+        for (int e = 0; e < VE; ++e) acc[e] *= alpha;
+        m_ref = m_new;
+        m_thr = m_new + kRaise;
       }
+      u32x4v pt;
+#pragma unroll
+      for (int a = 0; a < 2; ++a) {
+        float e[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          e[i] = __builtin_amdgcn_exp2f(x[a][i] - m_use);
+          l += e[i];
+        }
+        pt[2 * a] = Mat<T>::pack(e[0], e[1]);
+        pt[2 * a + 1] = Mat<T>::pack(e[2], e[3]);
+      }
+#pragma unroll
+      for (int e = 0; e < VW; ++e) {
+        u32x4v lo, hi;
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            lo[2 * a + j] = low_halves(vr[a][2 * j][e], vr[a][2 * j + 1][e]);
+            hi[2 * a + j] = high_halves(vr[a][2 * j][e], vr[a][2 * j + 1][e]);
+          }
+        acc[2 * e] = Mat<T>::mma16(lo, pt, acc[2 * e]);
+        acc[2 * e + 1] = Mat<T>::mma16(hi, pt, acc[2 * e + 1]);
+      }
+      if (more) load_v(t + STEP, nid);
+      id[0] = nid[0];
+      id[1] = nid[1];
     }
-  };
 
-  int t = begin + 32 * w;
-  int step = 0, ids = -1, id[2], nid[2];
-  if (t < end) {
-    ids = load_ids(t);
-    id[0] = __builtin_amdgcn_readlane(ids, 0);
-    id[1] = __builtin_amdgcn_readlane(ids, 1);
-    load_k(t, id);
-    load_v(t, id);
-  }
-  for (; t < end; t += kRound) {
-    const bool more = t + kRound < end;
-    if (more) {
-      if (++step == 32) {
-        step = 0;
-        ids = load_ids(t + kRound);
+    // ---- the waves' (m, l, o).  A wave that saw a NaN score has m = +inf, so that its
+    // weight is NaN; one that saw scores of -inf alone has l = NaN and counts only when no
+    // wave saw more.
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    if (l != l)
+      m_ref = __builtin_inff();
+    else if (m_ref == kNegInf && __any(some))
+      l = __builtin_nanf("");
+    if (g == 0) {
+      sm[w][n] = m_ref;
+      sl[w][n] = l;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int e = 0; e < VE; e += 4)
+        *(f32x4v*)&so[w][n][VE * (4 * g + i) + e] = f32x4v{acc[e][i], acc[e + 1][i], acc[e + 2][i], acc[e + 3][i]};
+    __syncthreads();
+    const int live = min(16, rows - 16 * tile);
+    const int64_t slot = 2 * (int64_t)blockIdx.x + (at_first > unit0 ? 0 : 1);
+    for (int u = tid; u < HW * live * (DT / 4); u += kThreads) {
+      const int hs = u / (live * (DT / 4)), r = u / (DT / 4) % live, d = 4 * (u % (DT / 4));
+      if (!FULL && d >= D) continue;
+      float m = kNegInf;
+#pragma unroll
+      for (int x = 0; x < WPH; ++x) m = fmaxf(m, sm[hs * WPH + x][r]);
+      f32x4v o = {0.f, 0.f, 0.f, 0.f};
+      float sum = 0.0f;
+#pragma unroll
+      for (int x = 0; x < WPH; ++x) {
+        const float mw = sm[hs * WPH + x][r];
+        if (mw == kNegInf && m != kNegInf) continue;
+        const float a = m == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(mw - m);
+        sum = fmaf(a, sl[hs * WPH + x][r], sum);
+        o += a * *(const f32x4v*)&so[hs * WPH + x][r][d];
       }
-      nid[0] = __builtin_amdgcn_readlane(ids, 2 * step);
-      nid[1] = __builtin_amdgcn_readlane(ids, 2 * step + 1);
-    }
-    f32x4v s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-    if constexpr (QL) asm volatile("" ::: "memory");  // read again each step
-#pragma unroll
-    for (int c = 0; c < KC; ++c) {
-      u32x4v q;
-      if constexpr (QL) q = *(const u32x4v*)&sq[n][16 * c + 4 * g]; else q = qr[c];
-#pragma unroll
-      for (int a = 0; a < 2; ++a) s[a] = Mat<T>::mma16(kr[a][c], q, s[a]);
-    }
-    if (more) load_k(t + kRound, nid);
-    const bool whole = id[0] >= 0 && id[1] >= 0 && t >= first && t + 32 <= end;
-    float x[2][4], mx = kNegInf;
-    const float gap = (float)(last - 1 - t - 4 * g);
-    each_score<8>(rule, [&](int i) { return s[i / 4][i % 4]; }, [&](int i, float y) { x[i / 4][i % 4] = y; });
-#pragma unroll
-    for (int a = 0; a < 2; ++a)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (p.alibi_slopes) x[a][i] = fmaf(-slope, gap - (float)(16 * a + i), x[a][i]);
-        if (!whole) {
-          const int tok = t + 16 * a + 4 * g + i;
-          const bool ok = id[a] >= 0 && tok >= first && tok < end;
-          x[a][i] = ok ? x[a][i] : kNegInf;
-          some |= ok;
+      if (direct) {
+        const float inv = begin < end && !(m == kNegInf && sum == 0.0f) ? 1.0f / sum : 0.0f;
+        T* dst = (T*)p.out + (int64_t)b * p.out_stride_b + ((h0 + hs) * rows + 16 * tile + r) * p.out_stride_h + d;
+        *(u32x2v*)dst = u32x2v{Mat<T>::pack(o[0] * inv, o[1] * inv), Mat<T>::pack(o[2] * inv, o[3] * inv)};
+      } else {
+        const int64_t i = slot * plan.slot_rows + hs * min(16, rows) + r;
+        *(f32x4v*)(plan.o + i * D + d) = o;
+        if (d == 0) {
+          plan.m[i] = m;
+          plan.l[i] = sum;
         }
-        mx = fmaxf(mx, x[a][i]);
-      }
-    some |= whole;
-    if (__any(mx > m_thr)) {
-      mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-      const float m_new = fmaxf(m_ref, mx);
-      m_use = m_new == kNegInf ? 0.0f : m_new;
-      const float alpha = __builtin_amdgcn_exp2f(m_ref - m_use);
-      l *= alpha;
-#pragma unroll
-      for (int e = 0; e < VE; ++e) acc[e] *= alpha;
-      m_ref = m_new;
-      m_thr = m_new + kRaise;
-    }
-    u32x4v pt;
-#pragma unroll
-    for (int a = 0; a < 2; ++a) {
-      float e[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        e[i] = __builtin_amdgcn_exp2f(x[a][i] - m_use);
-        l += e[i];
-      }
-      pt[2 * a] = Mat<T>::pack(e[0], e[1]);
-      pt[2 * a + 1] = Mat<T>::pack(e[2], e[3]);
-    }
-    if (!whole) {  // a masked value must not meet a zero weight
-#pragma unroll
-      for (int a = 0; a < 2; ++a)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int tok = t + 16 * a + 4 * g + j;
-          const bool ok = id[a] >= 0 && tok >= first && tok < end;
-#pragma unroll
-          for (int e = 0; e < VW; ++e) vr[a][j][e] = ok ? vr[a][j][e] : 0u;
-        }
-    }
-#pragma unroll
-    for (int e = 0; e < VW; ++e) {
-      u32x4v lo, hi;
-#pragma unroll
-      for (int a = 0; a < 2; ++a)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          lo[2 * a + j] = low_halves(vr[a][2 * j][e], vr[a][2 * j + 1][e]);
-          hi[2 * a + j] = high_halves(vr[a][2 * j][e], vr[a][2 * j + 1][e]);
-        }
-      acc[2 * e] = Mat<T>::mma16(lo, pt, acc[2 * e]);
-      acc[2 * e + 1] = Mat<T>::mma16(hi, pt, acc[2 * e + 1]);
-    }
-    if (more) load_v(t + kRound, nid);
-    id[0] = nid[0];
-    id[1] = nid[1];
-  }
-
-  // the four waves' (m, l, o) into one.  A wave that saw a NaN score has m = +inf, so
-  // that its weight is NaN; one that saw scores of -inf alone has l = NaN and counts
-  // only when no wave saw more.
-  l += __shfl_xor(l, 16, 64);
-  l += __shfl_xor(l, 32, 64);
-  if (l != l)
-    m_ref = __builtin_inff();
-  else if (m_ref == kNegInf && __any(some))
-    l = __builtin_nanf("");
-  if (g == 0) {
-    sm[w][n] = m_ref;
-    sl[w][n] = l;
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int e = 0; e < VE; e += 4)
-      *(f32x4v*)&so[w][n][VE * (4 * g + i) + e] = f32x4v{acc[e][i], acc[e + 1][i], acc[e + 2][i], acc[e + 3][i]};
-  __syncthreads();
-  const int live = min(16, rows - 16 * tile);
-  for (int u = threadIdx.x; u < live * (DT / 4); u += kThreads) {
-    const int r = u / (DT / 4), d = 4 * (u % (DT / 4));
-    if (!FULL && d >= D) continue;
-    float m = fmaxf(fmaxf(sm[0][r], sm[1][r]), fmaxf(sm[2][r], sm[3][r]));
-    f32x4v o = {0.f, 0.f, 0.f, 0.f};
-    float sum = 0.0f;
-#pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const float mw = sm[x][r];
-      if (mw == kNegInf && m != kNegInf) continue;
-      const float a = m == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(mw - m);
-      sum = fmaf(a, sl[x][r], sum);
-      o += a * *(const f32x4v*)&so[x][r][d];
-    }
-    const int hr = h * rows + 16 * tile + r;
-    if (direct) {
-      const float inv = begin < end && !(m == kNegInf && sum == 0.0f) ? 1.0f / sum : 0.0f;
-      T* dst = (T*)p.out + (int64_t)b * p.out_stride_b + hr * p.out_stride_h + d;
-      *(u32x2v*)dst = u32x2v{Mat<T>::pack(o[0] * inv, o[1] * inv), Mat<T>::pack(o[2] * inv, o[3] * inv)};
-    } else {
-      const int64_t i = ((int64_t)b * p.n_q_heads + hr) * part.splits + split;
-      *(f32x4v*)(part.o + i * D + d) = o;
-      if (d == 0) {
-        part.m[i] = m;
-        part.l[i] = sum;
       }
     }
+    at = stop;
+    if (at < at_end) __syncthreads();  // the next unit writes the same LDS
   }
 }
 
-// The splits of one row joined in their order: a workgroup a row.  First the splits'
-// weights into LDS, then thread (x, y) sums dims 4 x of every ny-th split, and the ny
-// sums are added in order.
-constexpr int kMaxSplits = 3072;
-
-template <typename T>
-__global__ __launch_bounds__(kThreads) void paged_merge_kernel(smaq_paged_params p, PagedPart part) {
-  __shared__ float sa[kMaxSplits];
-  __shared__ float so[kThreads][4], red[kThreads / 64];
+// One row whose steps went to several shares, joined in their order: a workgroup a
+// row.  First the partial results' weights into LDS, then thread (x, y) sums dims 4 x of
+// every ny-th, and the ny sums are added in order.
+template <typename T, int THREADS>
+__global__ __launch_bounds__(THREADS) void paged_merge_kernel(smaq_paged_params p, PagedPlan plan) {
+  __shared__ float sa[kMaxShares], sl[kMaxShares];
+  __shared__ float so[THREADS][4], red[2][THREADS / 64];
   const int tid = threadIdx.x, b = blockIdx.x / p.n_q_heads, hq = blockIdx.x % p.n_q_heads, D = p.head_dim;
-  int first, last;
-  visible(p, b, first, last);
-  const int64_t span = last - (first & ~15);
-  const int live = last > first ? (int)((span + part.split_len - 1) / part.split_len) : 0;
-  const int64_t i0 = (int64_t)blockIdx.x * part.splits;
-  float m = kNegInf;
-  for (int s = tid; s < live; s += kThreads) {
-    sa[s] = part.m[i0 + s];
-    m = fmaxf(m, sa[s]);
+  const int steps = unit_steps(p, b, 128 / plan.group);
+  if (steps == 0) return;
+  const int rows = p.n_q_heads / p.n_kv_heads, h = hq / rows, row = hq % rows;
+  const uint32_t all = plan.base[p.batch];
+  const uint32_t unit0 = plan.base[b] + (uint32_t)(h / plan.group * plan.tiles + row / 16) * steps;
+  const Deal deal(all, plan.shares);
+  const uint32_t g0 = deal.owner(unit0), g1 = deal.owner(unit0 + steps - 1);
+  if (g0 == g1) return;
+  const int live = g1 - g0 + 1, in_slot = h % plan.group * min(16, rows) + row % 16;
+  // the i-th: slot 1 of share g0, then slots 0
+  auto at = [&](int i) { return (int64_t)(2 * (g0 + i) + (i == 0)) * plan.slot_rows + in_slot; };
+  const int nx = D / 4, ny = THREADS / nx, x = tid % nx, y = tid / nx;
+  // everything is on its way before the first wait
+  constexpr int AHEAD = 8;
+  f32x4v v[AHEAD];
+#pragma unroll
+  for (int k = 0; k < AHEAD; ++k) v[k] = y + k * ny < live && y < ny ? *(const f32x4v*)(plan.o + at(y + k * ny) * D + 4 * x) : f32x4v{0.f, 0.f, 0.f, 0.f};
+  float m = kNegInf, l = 0.0f;
+  for (int i = tid; i < live; i += THREADS) {
+    sa[i] = plan.m[at(i)];
+    sl[i] = plan.l[at(i)];
+    m = fmaxf(m, sa[i]);
   }
   m = warp_max(m);
-  if ((tid & 63) == 0) red[tid >> 6] = m;
-  __syncthreads();
+  if (THREADS > 64) {
+    if ((tid & 63) == 0) red[0][tid >> 6] = m;
+    __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kThreads / 64; ++w) m = fmaxf(m, red[w]);
-  __syncthreads();
-  // a split of scores of -inf alone (m = -inf, l = NaN) counts only when all are
-  float l = 0.0f;
-  for (int s = tid; s < live; s += kThreads) {
-    const float ms = sa[s];
-    const float a = m == kNegInf ? 1.0f : (ms == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(ms - m));
-    sa[s] = a;
-    if (a != 0.0f) l = fmaf(a, part.l[i0 + s], l);  // NaN is not 0
+    for (int i = 0; i < THREADS / 64; ++i) m = fmaxf(m, red[0][i]);
+  }
+  for (int i = tid; i < live; i += THREADS) {
+    const float mi = sa[i];
+    const float a = m == kNegInf ? 1.0f : (mi == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(mi - m));
+    sa[i] = a;
+    if (a != 0.0f) l = fmaf(a, sl[i], l);  // NaN is not 0
   }
   l = warp_sum(l);
-  if ((tid & 63) == 0) red[tid >> 6] = l;
+  if ((tid & 63) == 0) red[1][tid >> 6] = l;
   __syncthreads();
   l = 0.0f;
 #pragma unroll
-  for (int w = 0; w < kThreads / 64; ++w) l += red[w];
-  const int nx = D / 4, ny = kThreads / nx, x = tid % nx, y = tid / nx;
+  for (int i = 0; i < THREADS / 64; ++i) l += red[1][i];
   f32x4v o = {0.f, 0.f, 0.f, 0.f};
-  if (y < ny) {
-    const float* src = part.o + i0 * D + 4 * x;
-#pragma unroll 8
-    for (int s = y; s < live; s += ny) {
-      const float a = sa[s];
-      const f32x4v v = *(const f32x4v*)(src + (int64_t)s * D);
+  auto add = [&](float a, const f32x4v& u) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] = a != 0.0f ? fmaf(a, v[e], o[e]) : o[e];
-    }
+    for (int e = 0; e < 4; ++e) o[e] = a != 0.0f ? fmaf(a, u[e], o[e]) : o[e];
+  };
+  if (y < ny) {
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k)
+      if (y + k * ny < live) add(sa[y + k * ny], v[k]);
+#pragma unroll 8
+    for (int i = y + AHEAD * ny; i < live; i += ny) add(sa[i], *(const f32x4v*)(plan.o + at(i) * D + 4 * x));
   }
   *(f32x4v*)so[tid] = o;
   __syncthreads();
   if (y != 0) return;
   for (int k = 1; k < ny; ++k) o += *(const f32x4v*)so[x + k * nx];
-  const float inv = live > 0 && !(m == kNegInf && l == 0.0f) ? 1.0f / l : 0.0f;
+  const float inv = m == kNegInf && l == 0.0f ? 0.0f : 1.0f / l;
   T* dst = (T*)p.out + (int64_t)b * p.out_stride_b + hq * p.out_stride_h + 4 * x;
   *(u32x2v*)dst = u32x2v{Mat<T>::pack(o[0] * inv, o[1] * inv), Mat<T>::pack(o[2] * inv, o[3] * inv)};
 }
@@ -386,43 +516,62 @@ int check_paged(const smaq_paged_params* p) {
   return SMAQ_OK;
 }
 
-// Splits of the longest sequence.  Enough workgroups for four rounds of the card (three
-// to a CU), but none of fewer than 256 tokens.
-PagedPart plan_splits(const smaq_paged_params* p) {
-  const int64_t longest = std::min<int64_t>(std::min<int64_t>(p->max_seq_len, (int64_t)p->max_blocks * p->block_size), kLongest);
-  int64_t span = p->window ? std::min<int64_t>(longest, (int64_t)p->window + 15) : longest;
-  span = std::max<int64_t>(span, 1);
+PagedPlan make_plan(const smaq_paged_params* p) {
   const int rows = p->n_q_heads / p->n_kv_heads;
-  const int64_t units = (int64_t)p->batch * p->n_kv_heads * ((rows + 15) / 16);
-  const int64_t want = kMaxSplits;
-  int64_t len = (span * units + want - 1) / want;
-  len = std::max<int64_t>((len + kRound - 1) / kRound * kRound, 256);
-  PagedPart part{nullptr, nullptr, nullptr, (int)((span + len - 1) / len), len};
-  return part;
+  PagedPlan plan{};
+  plan.tiles = (rows + 15) / 16;
+  const int64_t longest = std::min<int64_t>(std::min<int64_t>(p->max_seq_len, (int64_t)p->max_blocks * p->block_size), kLongest);
+  const int64_t span = p->window ? std::min<int64_t>(longest, (int64_t)p->window + 15) : longest;
+  const int64_t room = 256 * (p->head_dim <= 64 ? 4 : p->head_dim <= 128 ? 3 : 2);  // workgroups the card holds
+  const int64_t heads = (int64_t)p->n_kv_heads * plan.tiles * p->batch;
+  // four heads side by side while that leaves every workgroup four steps of 32 tokens (at
+  // 256 dims a row is long enough by itself)
+  const bool wide = p->head_dim <= 128 && p->n_kv_heads % 4 == 0 && (span + 31) / 32 * (heads / 4) >= 4 * room;
+  const int64_t most = wide ? (span + 31) / 32 * (heads / 4) : (span + 127) / 128 * heads;
+  if (span > 256 && most < (1ll << 31))
+    plan.shares = (int)std::max<int64_t>(1, std::min<int64_t>(room, most / kLeastSteps));
+  plan.group = wide && plan.shares ? 4 : 1;
+  plan.units = p->n_kv_heads / plan.group * plan.tiles;
+  plan.slot_rows = plan.group * std::min(16, rows);
+  return plan;
 }
 
-int64_t part_bytes(const smaq_paged_params* p, const PagedPart& part) {
-  if (part.splits == 1) return 0;
-  return (int64_t)p->batch * p->n_q_heads * part.splits * (p->head_dim + 2) * (int64_t)sizeof(float);
+int64_t plan_bytes(const smaq_paged_params* p, const PagedPlan& plan) {
+  if (plan.shares == 0) return 0;
+  const int64_t rows = 2 * (int64_t)plan.shares * plan.slot_rows;
+  return rows * (p->head_dim + 2) * (int64_t)sizeof(float) + ((int64_t)p->batch + 1) * (int64_t)sizeof(uint32_t);
+}
+
+template <typename T, int DT, int HW, bool WHOLE>
+void launch_paged(const smaq_paged_params& p, const ScoreRule& rule, const PagedPlan& plan, unsigned blocks, hipStream_t st) {
+  if (p.head_dim == DT)
+    paged_kernel<T, DT, true, HW, WHOLE><<<blocks, kThreads, 0, st>>>(p, rule, plan);
+  else
+    paged_kernel<T, DT, false, HW, WHOLE><<<blocks, kThreads, 0, st>>>(p, rule, plan);
 }
 
 template <typename T, int DT>
-void launch_paged(const smaq_paged_params& p, const ScoreRule& rule, const PagedPart& part, unsigned blocks, hipStream_t st) {
-  if (p.head_dim == DT)
-    paged_kernel<T, DT, true><<<blocks, kThreads, 0, st>>>(p, rule, part);
-  else
-    paged_kernel<T, DT, false><<<blocks, kThreads, 0, st>>>(p, rule, part);
+void launch_paged(const smaq_paged_params& p, const ScoreRule& rule, const PagedPlan& plan, unsigned blocks, hipStream_t st) {
+  if (plan.shares == 0) return launch_paged<T, DT, 1, true>(p, rule, plan, blocks, st);
+  if constexpr (DT <= 128)
+    if (plan.group == 4) return launch_paged<T, DT, 4, false>(p, rule, plan, blocks, st);
+  launch_paged<T, DT, 1, false>(p, rule, plan, blocks, st);
 }
 
 template <typename T>
-void launch_paged(const smaq_paged_params& p, const ScoreRule& rule, const PagedPart& part, unsigned blocks, hipStream_t st) {
-  if (p.head_dim <= 64)
-    launch_paged<T, 64>(p, rule, part, blocks, st);
-  else if (p.head_dim <= 128)
-    launch_paged<T, 128>(p, rule, part, blocks, st);
+void launch_paged(const smaq_paged_params& p, const ScoreRule& rule, const PagedPlan& plan, unsigned blocks, hipStream_t st) {
+  if (p.head_dim > 128)
+    launch_paged<T, 256>(p, rule, plan, blocks, st);
+  else if (p.head_dim > 64)
+    launch_paged<T, 128>(p, rule, plan, blocks, st);
   else
-    launch_paged<T, 256>(p, rule, part, blocks, st);
-  if (part.splits > 1) paged_merge_kernel<T><<<(unsigned)(p.batch * p.n_q_heads), kThreads, 0, st>>>(p, part);
+    launch_paged<T, 64>(p, rule, plan, blocks, st);
+  if (plan.shares <= 1) return;
+  const unsigned rows = (unsigned)(p.batch * p.n_q_heads);
+  if (rows <= 1024)
+    paged_merge_kernel<T, 256><<<rows, 256, 0, st>>>(p, plan);
+  else
+    paged_merge_kernel<T, 64><<<rows, 64, 0, st>>>(p, plan);
 }
 
 }  // namespace
@@ -431,7 +580,7 @@ void launch_paged(const smaq_paged_params& p, const ScoreRule& rule, const Paged
 extern "C" long long smaq_paged_workspace_bytes(const smaq_paged_params* p) {
   using namespace smaq;
   if (check_paged(p) != SMAQ_OK) return -1;
-  return p->batch ? part_bytes(p, plan_splits(p)) : 0;
+  return p->batch ? plan_bytes(p, make_plan(p)) : 0;
 }
 
 extern "C" int smaq_paged_attention(const smaq_paged_params* p, void* stream) {
@@ -449,25 +598,23 @@ extern "C" int smaq_paged_attention(const smaq_paged_params* p, void* stream) {
   SMAQ_REQUIRE(p->k_stride_t >= 0 && p->v_stride_t >= 0 && p->k_stride_t < (1ll << 26) && p->v_stride_t < (1ll << 26),
                "smaq_paged_attention: a token stride of %lld or %lld elements is not below 2^26", p->k_stride_t,
                p->v_stride_t);
-  PagedPart part = plan_splits(p);
-  const int64_t need = part_bytes(p, part);
+  PagedPlan plan = make_plan(p);
+  const int64_t need = plan_bytes(p, plan);
   SMAQ_REQUIRE(need == 0 || (p->workspace && p->workspace_bytes >= need && (uintptr_t)p->workspace % 16 == 0),
                "smaq_paged_attention: a 16-byte aligned workspace of %lld bytes is needed, got %lld", (long long)need,
                p->workspace_bytes);
-  const int64_t rows = (int64_t)p->batch * p->n_q_heads;
-  part.o = (float*)p->workspace;
-  if (part.splits > 1) {
-    part.m = part.o + rows * part.splits * p->head_dim;
-    part.l = part.m + rows * part.splits;
+  if (plan.shares) {
+    const int64_t rows = 2 * (int64_t)plan.shares * plan.slot_rows;
+    plan.o = (float*)p->workspace;
+    plan.m = plan.o + rows * p->head_dim;
+    plan.l = plan.m + rows;
+    plan.base = (uint32_t*)(plan.l + rows);
   }
-  const int tiles = (p->n_q_heads / p->n_kv_heads + 15) / 16;
-  const int64_t blocks = (int64_t)p->batch * part.splits * p->n_kv_heads * tiles;
-  SMAQ_REQUIRE(blocks <= 0x7fffffffll, "smaq_paged_attention: %lld workgroups are more than one launch takes",
-               (long long)blocks);
+  const int64_t blocks = plan.shares ? plan.shares : (int64_t)p->batch * plan.units;
   const ScoreRule rule = score_rule(p->scale, p->score_cap);
   if (p->dtype == SMAQ_F16)
-    launch_paged<_Float16>(*p, rule, part, (unsigned)blocks, (hipStream_t)stream);
+    launch_paged<_Float16>(*p, rule, plan, (unsigned)blocks, (hipStream_t)stream);
   else
-    launch_paged<bf16>(*p, rule, part, (unsigned)blocks, (hipStream_t)stream);
+    launch_paged<bf16>(*p, rule, plan, (unsigned)blocks, (hipStream_t)stream);
   return launch_status("smaq_paged_attention");
 }
