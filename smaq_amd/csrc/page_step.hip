@@ -20,29 +20,31 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxRequests = 8000;  // two sums each in 64 KB of LDS
-constexpr int64_t kIntMax = 0x7fffffff;
+constexpr uint32_t kMost = 0x7fffffff;  // lengths, sums and results stop here
 
 struct PageArgs {
   const void *context, *fresh;
   int context_wide, fresh_wide;
   int requests;
   int* table;
-  int width;
+  uint32_t width;
   const int* free_blocks;
-  int64_t n_free;
-  int bs;
-  int64_t tokens;
+  uint32_t n_free, bs, tokens;
   long long *slots, *positions;
   int *starts, *seq_lens, *status;
 };
 
-__device__ __forceinline__ int64_t length_at(const void* p, int wide, int b) {
-  const int64_t v = wide ? (int64_t)((const long long*)p)[b] : (int64_t)((const int*)p)[b];
-  return min(max(v, (int64_t)0), kIntMax);
+__device__ __forceinline__ uint32_t length_at(const void* p, int wide, int b) {
+  if (!wide) return (uint32_t)max(((const int*)p)[b], 0);
+  return (uint32_t)min(max(((const long long*)p)[b], 0ll), (long long)kMost);
 }
 
+__device__ __forceinline__ uint32_t add_to_most(uint32_t x, uint32_t y) { return min(x + y, kMost); }  // both up to kMost
+
+__device__ __forceinline__ uint32_t pages_of(uint32_t n, uint32_t bs) { return n / bs + (n % bs != 0); }
+
 // the last index i of the ascending s[0..n) with s[i] <= x (s[0] <= x)
-__device__ __forceinline__ int last_at_most(const int* s, int n, int x) {
+__device__ __forceinline__ int last_at_most(const uint32_t* s, int n, uint32_t x) {
   int lo = 0, hi = n;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
@@ -52,87 +54,102 @@ __device__ __forceinline__ int last_at_most(const int* s, int n, int x) {
 }
 
 __global__ __launch_bounds__(kThreads) void page_step_kernel(PageArgs a) {
-  extern __shared__ int lds[];
-  int* row0 = lds;                    // [requests + 1] first token of each request
-  int* page0 = lds + a.requests + 1;  // [requests + 1] first taken page of each request
-  __shared__ int64_t part[2][kThreads / 64];
-  __shared__ int64_t placed_all;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int n = a.requests, bs = a.bs;
+  extern __shared__ uint32_t lds[];
+  uint32_t* row0 = lds;                    // [requests + 1] first token of each request
+  uint32_t* page0 = lds + a.requests + 1;  // [requests + 1] first taken page of each request
+  __shared__ uint32_t part[2][kThreads / 64], placed_all;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = a.requests;
+  const uint32_t bs = a.bs;
   // each thread sums its run of requests, then a scan over the threads
   const int each = (n + kThreads - 1) / kThreads;
   const int b0 = min(n, tid * each), b1 = min(n, b0 + each);
-  int64_t sum_n = 0, sum_t = 0;
+  uint32_t sum_n = 0, sum_t = 0;
   for (int b = b0; b < b1; ++b) {
-    const int64_t c = length_at(a.context, a.context_wide, b), m = length_at(a.fresh, a.fresh_wide, b);
-    sum_n += m;
-    sum_t += (c + m + bs - 1) / bs - (c + bs - 1) / bs;
+    const uint32_t c = length_at(a.context, a.context_wide, b), m = length_at(a.fresh, a.fresh_wide, b);
+    sum_n = add_to_most(sum_n, m);
+    sum_t = add_to_most(sum_t, pages_of(c + m, bs) - pages_of(c, bs));
   }
-  int64_t in_n = sum_n, in_t = sum_t;
+  uint32_t in_n = sum_n, in_t = sum_t, run_n = 0, run_t = 0;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
-    const int64_t x = __shfl_up(in_n, o, 64), y = __shfl_up(in_t, o, 64);
-    if (lane >= o) { in_n += x; in_t += y; }
+    const uint32_t x = __shfl_up(in_n, o, 64), y = __shfl_up(in_t, o, 64);
+    if (lane >= o) {
+      in_n = add_to_most(in_n, x);
+      in_t = add_to_most(in_t, y);
+    }
   }
-  if (lane == 63) { part[0][wave] = in_n; part[1][wave] = in_t; }
+  const uint32_t up_n = __shfl_up(in_n, 1, 64), up_t = __shfl_up(in_t, 1, 64);
+  if (lane) {
+    run_n = up_n;
+    run_t = up_t;
+  }
+  if (lane == 63) {
+    part[0][wave] = in_n;
+    part[1][wave] = in_t;
+  }
   if (tid == 0) placed_all = 0;
   __syncthreads();
-  int64_t run_n = in_n - sum_n, run_t = in_t - sum_t, total_n = 0, total_t = 0;
+  uint32_t total_n = 0, total_t = 0, wave_n = 0, wave_t = 0;
 #pragma unroll
   for (int w = 0; w < kThreads / 64; ++w) {
-    if (w < wave) { run_n += part[0][w]; run_t += part[1][w]; }
-    total_n += part[0][w];
-    total_t += part[1][w];
+    if (w == wave) {
+      wave_n = total_n;
+      wave_t = total_t;
+    }
+    total_n = add_to_most(total_n, part[0][w]);
+    total_t = add_to_most(total_t, part[1][w]);
   }
-  int64_t placed = 0;  // tokens of this thread's requests that get a slot (workgroup 0 reports them)
+  run_n = add_to_most(run_n, wave_n);
+  run_t = add_to_most(run_t, wave_t);
+  uint32_t placed = 0;  // tokens of this thread's requests that get a slot (workgroup 0 reports them)
   for (int b = b0; b < b1; ++b) {
-    row0[b] = (int)min(run_n, kIntMax);
-    page0[b] = (int)min(run_t, kIntMax);
-    const int64_t c = length_at(a.context, a.context_wide, b), m = length_at(a.fresh, a.fresh_wide, b);
-    const int64_t held = (c + bs - 1) / bs, taken = (c + m + bs - 1) / bs - held;
+    row0[b] = run_n;
+    page0[b] = run_t;
+    const uint32_t c = length_at(a.context, a.context_wide, b), m = length_at(a.fresh, a.fresh_wide, b);
+    const uint32_t held = pages_of(c, bs), taken = pages_of(c + m, bs) - held;
     if (blockIdx.x == 0) {
-      const int64_t pages = min((int64_t)a.width, held + min(max(a.n_free - run_t, (int64_t)0), taken));
-      const int64_t rows = min(max(a.tokens - run_n, (int64_t)0), m);
-      int64_t ok = min(max(pages * bs - c, (int64_t)0), rows);
+      const uint32_t got = min(a.n_free > run_t ? a.n_free - run_t : 0u, taken);
+      const uint64_t room = (uint64_t)min(a.width, held + got) * bs;
+      const uint32_t rows = min(a.tokens > run_n ? a.tokens - run_n : 0u, m);
+      uint32_t ok = room > c ? (uint32_t)min(room - c, (uint64_t)rows) : 0u;
       if (c % bs && c / bs < a.width && a.table[(int64_t)b * a.width + c / bs] < 0) ok -= min(ok, bs - c % bs);
       placed += ok;
     }
-    run_n += m;
-    run_t += taken;
+    run_n = add_to_most(run_n, m);
+    run_t = add_to_most(run_t, taken);
   }
   if (tid == 0) {
-    row0[n] = (int)min(total_n, kIntMax);
-    page0[n] = (int)min(total_t, kIntMax);
+    row0[n] = total_n;
+    page0[n] = total_t;
   }
-  if (blockIdx.x == 0 && placed) atomicAdd((unsigned long long*)&placed_all, (unsigned long long)placed);
+  if (blockIdx.x == 0 && placed) atomicAdd(&placed_all, placed);
   __syncthreads();
   if (blockIdx.x == 0 && tid == 0) {
-    a.status[0] = (int)min(total_t, kIntMax);
-    a.status[1] = (int)min(total_n - placed_all, kIntMax);
+    a.status[0] = (int)total_t;
+    a.status[1] = (int)(total_n - placed_all);
   }
-  const int64_t stride = (int64_t)gridDim.x * kThreads, first = (int64_t)blockIdx.x * kThreads + tid;
-  for (int64_t b = first; b <= n; b += stride) {
-    a.starts[b] = row0[b];
-    if (b < n)
-      a.seq_lens[b] = (int)min(length_at(a.context, a.context_wide, (int)b) + length_at(a.fresh, a.fresh_wide, (int)b),
-                               kIntMax);
+  const uint32_t stride = gridDim.x * kThreads, first = blockIdx.x * kThreads + tid;
+  for (uint32_t b = first; b <= (uint32_t)n; b += stride) {
+    a.starts[b] = (int)row0[b];
+    if (b < (uint32_t)n)
+      a.seq_lens[b] = (int)min(length_at(a.context, a.context_wide, (int)b) + length_at(a.fresh, a.fresh_wide, (int)b), kMost);
   }
   // taken pages: entry e of the free list goes to its request's next column
-  for (int64_t e = first; e < min(total_t, kIntMax); e += stride) {
-    const int b = last_at_most(page0, n, (int)e);
-    const int64_t c = length_at(a.context, a.context_wide, b);
-    const int64_t col = (c + bs - 1) / bs + (e - page0[b]);
+  for (uint32_t e = first; e < total_t; e += stride) {
+    const int b = last_at_most(page0, n, e);
+    const uint64_t col = (uint64_t)pages_of(length_at(a.context, a.context_wide, b), bs) + (e - page0[b]);
     if (col < a.width) a.table[(int64_t)b * a.width + col] = e < a.n_free ? a.free_blocks[e] : -1;
   }
-  for (int64_t i = first; i < a.tokens; i += stride) {
-    int64_t slot = -1, pos = 0;
-    if (i < min(total_n, kIntMax)) {
-      const int b = last_at_most(row0, n, (int)i);
-      const int64_t c = length_at(a.context, a.context_wide, b);
+  for (uint32_t i = first; i < a.tokens; i += stride) {
+    int64_t slot = -1;
+    uint32_t pos = 0;
+    if (i < total_n) {
+      const int b = last_at_most(row0, n, i);
+      const uint32_t c = length_at(a.context, a.context_wide, b);
       pos = c + (i - row0[b]);
-      const int64_t col = pos / bs, held = (c + bs - 1) / bs;
+      const uint32_t col = pos / bs, held = pages_of(c, bs);
       if (col < a.width) {
-        const int64_t e = page0[b] + (col - held);
+        const uint64_t e = (uint64_t)page0[b] + (col - held);
         const int blk = col < held ? a.table[(int64_t)b * a.width + col] : (e < a.n_free ? a.free_blocks[e] : -1);
         if (blk >= 0) slot = (int64_t)blk * bs + pos % bs;
       }
@@ -153,7 +170,7 @@ extern "C" int smaq_page_step(const void* context_lens, int context_bytes, const
   SMAQ_REQUIRE(requests >= 0 && requests <= kMaxRequests, "smaq_page_step: %d requests are not in 0..%d", requests,
                kMaxRequests);
   SMAQ_REQUIRE(block_size >= 1 && block_size <= 65536 && max_blocks >= 0 && n_free >= 0 && tokens >= 0 &&
-                   n_free <= kIntMax && tokens <= kIntMax,
+                   n_free <= (long long)kMost && tokens <= (long long)kMost,
                "smaq_page_step: bad sizes (block_size %d, max_blocks %d, %lld free, %lld tokens)", block_size,
                max_blocks, n_free, tokens);
   SMAQ_REQUIRE((context_bytes == 4 || context_bytes == 8) && (new_bytes == 4 || new_bytes == 8),
@@ -161,10 +178,11 @@ extern "C" int smaq_page_step(const void* context_lens, int context_bytes, const
   SMAQ_REQUIRE((!requests || (context_lens && new_lens && seq_lens)) && (!requests || !max_blocks || block_table) &&
                    (!n_free || free_blocks) && (!tokens || (slot_mapping && positions)) && query_start_loc && status,
                "smaq_page_step: null pointer");
-  PageArgs a{context_lens, new_lens, context_bytes == 8, new_bytes == 8, requests, block_table, max_blocks,
-             free_blocks, n_free, block_size, tokens, slot_mapping, positions, query_start_loc, seq_lens, status};
-  // four tokens a thread while there are many; one workgroup each 256 otherwise
-  const int64_t groups = std::min<int64_t>(std::max<int64_t>((tokens + kThreads - 1) / kThreads, (requests + 255) / 256 + 1), 256);
+  PageArgs a{context_lens, new_lens, context_bytes == 8, new_bytes == 8, requests, block_table, (uint32_t)max_blocks,
+             free_blocks, (uint32_t)n_free, (uint32_t)block_size, (uint32_t)tokens, slot_mapping, positions,
+             query_start_loc, seq_lens, status};
+  // a token or request a thread, up to one workgroup a CU
+  const int64_t groups = std::min<int64_t>((std::max<int64_t>(tokens, requests + 1) + kThreads - 1) / kThreads, 256);
   const size_t bytes = 2 * sizeof(int) * (size_t)(requests + 1);
   page_step_kernel<<<(unsigned)std::max<int64_t>(groups, 1), kThreads, bytes, (hipStream_t)stream>>>(a);
   return launch_status("smaq_page_step");
