@@ -415,20 +415,28 @@ __global__ __launch_bounds__(kThreads, 2) void packed_kernel(smaq_packed_params 
     for (int i = 0; i < 16; ++i) z = fmaf(acc[db][i], 0.0f, z);
   if (__syncthreads_or(live && z != z)) run(std::true_type{});
 
-  if (unit >= blocks * g || row >= T_all || !(live || p.zero_rest)) return;
+  // ---- the result, turned in LDS (every wave is done with its tiles) so that it leaves in
+  // whole rows
+  __syncthreads();
   l += __shfl_xor(l, 32, 64);
   const float inv = live ? 1.0f / l : 0.0f;
-  T* dst = (T*)p.out + (int64_t)row * p.out_stride_t + hq * p.out_stride_h + 4 * half;
+  char* turned = lds + w * 32 * RS;
 #pragma unroll
   for (int db = 0; db < DB; ++db)
 #pragma unroll
     for (int i = 0; i < 16; i += 4) {
-      const int d = 32 * db + 8 * (i / 4);
-      if (FULL || d < D) {
-        const u32x2v y = {Mat<T>::pack(acc[db][i] * inv, acc[db][i + 1] * inv), Mat<T>::pack(acc[db][i + 2] * inv, acc[db][i + 3] * inv)};
-        *(u32x2v*)(dst + d) = live ? y : u32x2v{0, 0};
-      }
+      const u32x2v y = {Mat<T>::pack(acc[db][i] * inv, acc[db][i + 1] * inv), Mat<T>::pack(acc[db][i + 2] * inv, acc[db][i + 3] * inv)};
+      *(u32x2v*)(turned + n * RS + 16 * ((4 * db + i / 4) ^ (n & (UPR < 16 ? 7 : 15))) + 8 * half) = live ? y : u32x2v{0, 0};
     }
+  const unsigned long long rows_live = __ballot(live);
+  if (unit >= blocks * g) return;
+#pragma unroll
+  for (int k = 0; k < 32 * UPR / 64; ++k) {
+    const int r = (64 * k + lane) / UPR, u = lane % UPR;
+    const u32x4v y = *(const u32x4v*)(turned + r * RS + 16 * (u ^ (r & (UPR < 16 ? 7 : 15))));
+    if (32 * tb + r < T_all && (p.zero_rest || ((rows_live >> r) & 1)) && (FULL || 8 * u < D))
+      *(u32x4v*)((T*)p.out + (int64_t)(32 * tb + r) * p.out_stride_t + hq * p.out_stride_h + 8 * u) = y;
+  }
 }
 
 template <typename T, int DT, bool FULL>
