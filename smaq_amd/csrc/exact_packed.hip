@@ -74,7 +74,7 @@ __device__ __forceinline__ int wave_max(int v) {
 }
 
 template <typename T, int DT, bool FULL, bool CAP, bool ALIBI>
-__global__ __launch_bounds__(kThreads, 2) void packed_kernel(smaq_packed_params p, ScoreRule rule, int blocks) {
+__global__ __launch_bounds__(kThreads, DT == 64 ? 3 : 2) void packed_kernel(smaq_packed_params p, ScoreRule rule, int blocks) {
   constexpr int KT = DT == 256 ? 32 : 64;  // keys per tile
   constexpr int KB = KT / 32;              // 32-key blocks
   constexpr int KS = DT / 16;              // k steps of a product over the head dim
@@ -93,9 +93,16 @@ __global__ __launch_bounds__(kThreads, 2) void packed_kernel(smaq_packed_params 
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = p.n_q_heads / p.n_kv_heads, D = p.head_dim, T_all = (int)p.n_tokens;
   const int h = blockIdx.x % p.n_kv_heads;
-  // the last tokens first: with a causal mask they have the most keys
+  // The last tokens first: with a causal mask they have the most keys.  A grid that the card
+  // holds at once puts the i-th workgroup of every 256 on the same CU: every second 256 runs
+  // the other way round, so that a CU gets long and short ones.
   const int groups = (blocks * g + 3) / 4;
-  const int unit = 4 * (groups - 1 - (int)(blockIdx.x / p.n_kv_heads)) + w;
+  int rank = blockIdx.x / p.n_kv_heads;
+  if (gridDim.x <= 256 * (DT == 64 ? 3 : 2) && 256 % p.n_kv_heads == 0) {
+    const int per = 256 / p.n_kv_heads, first = rank / per * per;
+    if (rank / per & 1) rank = first + min(groups, first + per) - 1 - rank;
+  }
+  const int unit = 4 * (groups - 1 - rank) + w;
   const int tb = unit / g, hq = h * g + unit % g;
   const int row = 32 * tb + n;
 
