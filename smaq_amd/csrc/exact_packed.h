@@ -1,4 +1,5 @@
-// Attention over a step's own exact tokens (smaq_packed_attention).
+// Attention over a step's own exact tokens: the kernel of smaq_packed_attention,
+// instantiated per type (exact_packed_f16.hip, exact_packed_bf16.hip).
 //
 // 4 D operations per visible pair and head over a few bytes per token: the matrix
 // cores bound it, then the vector unit (the exponentials) and LDS (operand reads).
@@ -17,7 +18,9 @@
 //                              8 + 4 h ..), A = V^T by transposing LDS reads
 //
 // Tiles of 64 keys (32 at 256 dims) are copied global -> LDS one tile ahead, 16-byte
-// units placed by an XOR of the row so that operand reads meet no bank twice.
+// units placed by an XOR of the row so that operand reads meet no bank twice.  Small
+// grids have two groups of four waves per workgroup (KG = 2), each with every second
+// tile; their results are joined in LDS.
 //
 // Masks.  A tile that every row of a wave sees whole takes no mask.  In others a
 // masked score becomes -inf after scale, cap and bias, so NaN there is dropped; a
@@ -25,6 +28,8 @@
 // shows as a result that is not finite: such a workgroup runs again with the masked
 // tiles' numbers that are not finite taken out of the product (the other rows keep
 // their bits) and added key by key to the rows that see them.
+#pragma once
+
 #include <math.h>
 
 #include <type_traits>
@@ -73,8 +78,8 @@ __device__ __forceinline__ int wave_max(int v) {
   return __builtin_amdgcn_readfirstlane(v);
 }
 
-template <typename T, int DT, bool FULL, bool CAP, bool ALIBI>
-__global__ __launch_bounds__(kThreads, DT == 64 ? 3 : 2) void packed_kernel(smaq_packed_params p, ScoreRule rule, int blocks) {
+template <typename T, int DT, bool FULL, bool CAP, bool ALIBI, int KG>
+__global__ __launch_bounds__(KG * kThreads, DT == 64 && KG == 1 ? 3 : 2) void packed_kernel(smaq_packed_params p, ScoreRule rule, int blocks) {
   constexpr int KT = DT == 256 ? 32 : 64;  // keys per tile
   constexpr int KB = KT / 32;              // 32-key blocks
   constexpr int KS = DT / 16;              // k steps of a product over the head dim
@@ -87,10 +92,13 @@ __global__ __launch_bounds__(kThreads, DT == 64 ? 3 : 2) void packed_kernel(smaq
   // 1.17 -> 1.12 ms; without a cap at up to 128 dims they are better left alone (2.14 -> 2.11
   // ms, 8192 tokens of 8 / 8 heads 231 -> 214 us).
   constexpr bool PRIO = CAP || DT == 256;
-  __shared__ __attribute__((aligned(16))) char lds[4 * TILE];  // two buffers of (keys, values)
+  __shared__ __attribute__((aligned(16))) char all_lds[KG * 4 * TILE];  // of each key group two buffers of (keys, values)
   __shared__ int span[4][4];
-  const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, half = lane >> 5;
+  __shared__ float joined[KG == 2 ? 4 : 1][2][64];
+  const int tid = threadIdx.x % kThreads, lane = tid & 63, n = lane & 31, half = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int kg = KG == 1 ? 0 : __builtin_amdgcn_readfirstlane((int)threadIdx.x / kThreads);
+  char* lds = all_lds + kg * 4 * TILE;
   const int g = p.n_q_heads / p.n_kv_heads, D = p.head_dim, T_all = (int)p.n_tokens;
   const int h = blockIdx.x % p.n_kv_heads;
   // The last tokens first: with a causal mask they have the most keys.  A grid that the card
@@ -98,7 +106,7 @@ __global__ __launch_bounds__(kThreads, DT == 64 ? 3 : 2) void packed_kernel(smaq
   // the other way round, so that a CU gets long and short ones.
   const int groups = (blocks * g + 3) / 4;
   int rank = blockIdx.x / p.n_kv_heads;
-  if (gridDim.x <= 256 * (DT == 64 ? 3 : 2) && 256 % p.n_kv_heads == 0) {
+  if (KG == 1 && gridDim.x <= 256 * (DT == 64 ? 3 : 2) && 256 % p.n_kv_heads == 0) {
     const int per = 256 / p.n_kv_heads, first = rank / per * per;
     if (rank / per & 1) rank = first + min(groups, first + per) - 1 - rank;
   }
@@ -259,9 +267,11 @@ __global__ __launch_bounds__(kThreads, DT == 64 ? 3 : 2) void packed_kernel(smaq
     for (int db = 0; db < DB; ++db) acc[db] = f32x16v{};
     m_ref = m_thr = kNegInf;
     m_use = l = 0.0f;
-    if (k_lo < k_hi) copy_tile(k_lo, 0);
+    // of every KG tiles this wave's group takes the kg-th
+    const int k_first = kg == 0 ? k_lo : next_tile(k_lo);
+    if (k_lo < k_hi && k_first < k_hi) copy_tile(k_first, 0);
     int buf = 0;
-    for (int k = k_lo; k < k_hi; buf ^= 1) {
+    for (int k = k_lo, k_mine = k_first; k < k_hi; buf ^= 1) {
       // this thread's copies have landed, then everyone's; everyone is done with the
       // other buffer
       asm volatile("" ::: "memory");
@@ -269,10 +279,11 @@ __global__ __launch_bounds__(kThreads, DT == 64 ? 3 : 2) void packed_kernel(smaq
       asm volatile("" ::: "memory");
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
-      const int k_next = next_tile(k);
-      if (k_next < k_hi) copy_tile(k_next, buf ^ 1);
-      const int k0 = k;
-      k = k_next;
+      const int k0 = k_mine;
+      k = next_tile(k);
+      if (KG == 2) k = next_tile(k);
+      k_mine = kg == 0 ? k : next_tile(k);
+      if (k_mine < k_hi) copy_tile(k_mine, buf ^ 1);
       if (k0 >= w_hi || k0 + KT <= w_lo || (k0 >= w_gap0 && k0 + KT <= w_gap1)) continue;
       const int kt = buf * 2 * TILE + koff, vt = buf * 2 * TILE + TILE + voff;
       f32x16v s[KB];
@@ -426,8 +437,34 @@ __global__ __launch_bounds__(kThreads, DT == 64 ? 3 : 2) void packed_kernel(smaq
   // whole rows
   __syncthreads();
   l += __shfl_xor(l, 32, 64);
+  char* turned = all_lds + w * (KG == 1 ? 32 * RS : DB * 4096);
+  if constexpr (KG == 2) {
+    // the second key group's (m, l, o) into the first's, register by register
+    f32x4v* other = (f32x4v*)turned + lane;
+    if (kg == 1) {
+      joined[w][0][lane] = m_ref;
+      joined[w][1][lane] = l;
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4)
+          other[64 * (4 * db + i / 4)] = f32x4v{acc[db][i], acc[db][i + 1], acc[db][i + 2], acc[db][i + 3]};
+    }
+    __syncthreads();
+    if (kg == 1) return;
+    const float m1 = joined[w][0][lane], m = fmaxf(m_ref, m1);
+    const float mu = m == kNegInf ? 0.0f : m, a0 = __builtin_amdgcn_exp2f(m_ref - mu), a1 = __builtin_amdgcn_exp2f(m1 - mu);
+    l = l * a0 + joined[w][1][lane] * a1;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) {
+        const f32x4v o = other[64 * (4 * db + i / 4)];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[db][i + e] = acc[db][i + e] * a0 + o[e] * a1;
+      }
+  }
   const float inv = live ? 1.0f / l : 0.0f;
-  char* turned = lds + w * 32 * RS;
 #pragma unroll
   for (int db = 0; db < DB; ++db)
 #pragma unroll
@@ -446,17 +483,30 @@ __global__ __launch_bounds__(kThreads, DT == 64 ? 3 : 2) void packed_kernel(smaq
   }
 }
 
+template <typename T, int DT, bool FULL, bool CAP, bool ALIBI>
+void launch_packed(const smaq_packed_params& p, const ScoreRule& rule, unsigned grid, int blocks, hipStream_t st) {
+  // A grid that leaves the card's waves idle, or that is as long as its longest workgroup
+  // (two a CU, long documents), gives every unit two groups of waves, which take the key
+  // tiles in turn: one prompt of 1500 tokens 43 -> 34 us, 8192 tokens of 8 / 8 heads 214 ->
+  // 163; but four prompts of 512 23 -> 32, and 3000 tokens 91 -> 105 us.
+  const bool split = (grid <= 256 && p.n_tokens > 256) || (grid <= 512 && p.n_tokens >= 768ll * p.n_docs);
+  if (split)
+    packed_kernel<T, DT, FULL, CAP, ALIBI, 2><<<grid, 2 * kThreads, 0, st>>>(p, rule, blocks);
+  else
+    packed_kernel<T, DT, FULL, CAP, ALIBI, 1><<<grid, kThreads, 0, st>>>(p, rule, blocks);
+}
+
 template <typename T, int DT, bool FULL>
 void launch_packed(const smaq_packed_params& p, const ScoreRule& rule, unsigned grid, int blocks, hipStream_t st) {
   if (p.score_cap > 0.0f) {
     if (p.alibi_slopes)
-      packed_kernel<T, DT, FULL, true, true><<<grid, kThreads, 0, st>>>(p, rule, blocks);
+      launch_packed<T, DT, FULL, true, true>(p, rule, grid, blocks, st);
     else
-      packed_kernel<T, DT, FULL, true, false><<<grid, kThreads, 0, st>>>(p, rule, blocks);
+      launch_packed<T, DT, FULL, true, false>(p, rule, grid, blocks, st);
   } else if (p.alibi_slopes) {
-    packed_kernel<T, DT, FULL, false, true><<<grid, kThreads, 0, st>>>(p, rule, blocks);
+    launch_packed<T, DT, FULL, false, true>(p, rule, grid, blocks, st);
   } else {
-    packed_kernel<T, DT, FULL, false, false><<<grid, kThreads, 0, st>>>(p, rule, blocks);
+    launch_packed<T, DT, FULL, false, false>(p, rule, grid, blocks, st);
   }
 }
 
@@ -482,37 +532,3 @@ void launch_packed(const smaq_packed_params& p, const ScoreRule& rule, unsigned 
 
 }  // namespace
 }  // namespace smaq
-
-extern "C" int smaq_packed_attention(const smaq_packed_params* p, void* stream) {
-  using namespace smaq;
-  SMAQ_REQUIRE(p, "smaq_packed_attention: null parameters");
-  SMAQ_REQUIRE(p->n_tokens >= 0 && p->n_tokens <= 0x7fffff00ll && p->n_docs >= 0 && p->n_q_heads > 0 &&
-                   p->n_kv_heads > 0 && p->n_q_heads % p->n_kv_heads == 0 && p->n_q_heads <= 65536,
-               "smaq_packed_attention: bad shape (%lld tokens, %d documents, %d heads over %d)", p->n_tokens, p->n_docs,
-               p->n_q_heads, p->n_kv_heads);
-  SMAQ_REQUIRE(p->head_dim > 0 && p->head_dim <= 256 && p->head_dim % 8 == 0,
-               "smaq_packed_attention: head_dim %d is not a multiple of 8 up to 256", p->head_dim);
-  SMAQ_REQUIRE(p->window >= 0 && p->score_cap >= 0.0f && p->score_cap < 1e30f && p->scale == p->scale,
-               "smaq_packed_attention: window %d, score_cap %g and scale %g must be numbers of 0 or more, finite and "
-               "a number", p->window, (double)p->score_cap, (double)p->scale);
-  if (p->dtype != SMAQ_F16 && p->dtype != SMAQ_BF16) {
-    set_error("smaq_packed_attention: unsupported dtype %d", p->dtype);
-    return SMAQ_EUNSUPPORTED;
-  }
-  if (p->n_tokens == 0) return SMAQ_OK;
-  SMAQ_REQUIRE(p->q && p->k && p->v && p->out && (!p->n_docs || p->starts), "smaq_packed_attention: null pointer");
-  SMAQ_REQUIRE(rows_on_16(p->q, p->q_stride_t, p->q_stride_h) && rows_on_16(p->k, p->k_stride_t, p->k_stride_h) &&
-                   rows_on_16(p->v, p->v_stride_t, p->v_stride_h) && rows_on_16(p->out, p->out_stride_t, p->out_stride_h),
-               "smaq_packed_attention: rows must start on 16 bytes");
-  // the kernel gives the scale's sign, and a scale of 0, to the queries
-  const ScoreRule rule = score_rule(p->scale == 0.0f ? 1.0f : fabsf(p->scale), p->score_cap);
-  const int blocks = (int)((p->n_tokens + 31) / 32), g = p->n_q_heads / p->n_kv_heads;
-  const int64_t grid = ((int64_t)blocks * g + 3) / 4 * p->n_kv_heads;
-  SMAQ_REQUIRE((int64_t)blocks * g < 0x7ffffff0ll && grid <= 0x7fffffffll,
-               "smaq_packed_attention: %lld workgroups are more than one launch takes", (long long)grid);
-  if (p->dtype == SMAQ_F16)
-    launch_packed<_Float16>(*p, rule, (unsigned)grid, blocks, (hipStream_t)stream);
-  else
-    launch_packed<bf16>(*p, rule, (unsigned)grid, blocks, (hipStream_t)stream);
-  return launch_status("smaq_packed_attention");
-}

@@ -330,6 +330,42 @@ def test_packed_long_documents(dev, dtype):
     _check_packed(dev, [3001], 8, 8, 64, dtype, seed=5, cap=30.0, heads=(0, 5))
 
 
+@pytest.mark.parametrize("lens", [[1] * 62, [1] * 63, [1] * 64, [2] * 100 + [0] * 80 + [130] + [1] * 50, [0] * 200 + [70],
+                                  [300] + [0] * 70, [33, 0, 0, 31] * 30, [0] * 5000 + [3, 200, 1]])
+def test_packed_many_documents(dev, lens):
+    """Below and above the 63 documents whose starts one load holds, and runs of empty ones."""
+    _check_packed(dev, lens, 2, 1, 128, torch.bfloat16, seed=21)
+    _check_packed(dev, lens, 2, 2, 64, torch.float16, seed=22, window=9, prefix=[min(n, 5) for n in lens])
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("hq,hkv,lens", [(8, 8, [500]), (4, 2, [1100, 900]), (8, 2, [2048]), (2, 1, [257]),
+                                         (8, 8, [1000, 40, 1100])])
+def test_packed_key_groups(dev, D, hq, hkv, lens):
+    """Grids of a workgroup or two a CU, whose units have two groups of waves over the keys: causal and not, with a
+    gap between prefix and window, and values that are not finite."""
+    heads = (0, hq - 1)
+    _check_packed(dev, lens, hq, hkv, D, torch.bfloat16, seed=23, heads=heads)
+    _check_packed(dev, lens, hq, hkv, D, torch.float16, seed=24, causal=False, cap=30.0, heads=heads)
+    _check_packed(dev, lens, hq, hkv, D, torch.bfloat16, seed=25, prefix=[50] * len(lens), window=70, heads=heads)
+    q, k, v = _qkv(dev, sum(lens), hq, hkv, D, torch.bfloat16, 26)
+    starts, at = _starts(lens, dev), lens[0] - 20
+    clean = S.compute_packed_attention(q, k, v, starts)
+    bad = v.clone()
+    bad[at:lens[0]] = float("nan")
+    got = S.compute_packed_attention(q, k, bad, starts)
+    assert torch.equal(got[:at], clean[:at]) and torch.equal(got[lens[0]:], clean[lens[0]:])
+    assert bool(torch.isnan(got[at:lens[0]]).all())
+
+
+def test_packed_results_do_not_change_from_run_to_run(dev):
+    q, k, v = _qkv(dev, 3000, 8, 2, 128, torch.bfloat16, 27)
+    starts = _starts([1700, 1300], dev)
+    ref = S.compute_packed_attention(q, k, v, starts, score_cap=50.0)
+    for _ in range(3):
+        assert torch.equal(S.compute_packed_attention(q, k, v, starts, score_cap=50.0), ref)
+
+
 def test_packed_one_token(dev):
     q, k, v = _qkv(dev, 1, 4, 2, 128, torch.bfloat16, 6)
     out = S.compute_packed_attention(q, k, v, torch.tensor([0, 1], device=dev))
@@ -472,6 +508,89 @@ def test_paged_masks_caps_and_layouts(dev, D, kw):
 def test_paged_long_sequences(dev, dtype):
     _check_paged(dev, [20011], 4, 1, 128, dtype, seed=3)
     _check_paged(dev, [9000, 5, 4096, 12345], 7, 1, 128, dtype, seed=4, cap=50.0)
+
+
+@pytest.mark.parametrize("B", [63, 65, 300, 5000])
+def test_paged_many_sequences(dev, B):
+    """Shares that begin and end in any sequence, empty ones among them; every sequence has one page of its own, and a
+    few have forty."""
+    g = torch.Generator().manual_seed(B)
+    lens = torch.randint(0, 17, (B,), generator=g)
+    lens[torch.randint(0, B, (6,), generator=g)] = 640
+    lens[0], lens[-1] = 0, 0
+    bs, hkv, hq, D = 16, 4, 8, 64
+    kv = torch.randn(2, B + 40, bs, hkv, D, generator=_gen(B), device=dev).half()
+    table = torch.full((B, 40), -1, dtype=torch.int32)
+    table[:, 0] = torch.arange(B)
+    for b in (lens == 640).nonzero().flatten().tolist():
+        table[b] = torch.randperm(B + 40, generator=g)[:40].int()
+    q = torch.randn(B, hq, D, generator=_gen(B + 1), device=dev).half()
+    out = S.compute_paged_attention(q, kv[0], kv[1], table.to(dev), lens.to(dev), 640)
+    again = S.compute_paged_attention(q, kv[0], kv[1], table.to(dev), lens.to(dev).int(), 640)
+    assert torch.equal(out, again)
+    tab = table.to(dev).long()
+    for b in range(B):
+        n = int(lens[b])
+        if n == 0:
+            assert bool((out[b] == 0).all())
+            continue
+        if B > 400 and n < 640 and b % 50:
+            continue
+        j = torch.arange(n, device=dev)
+        for h in (0, hq - 1):
+            k, v = (kv[i][tab[b][j // bs], j % bs, h * hkv // hq] for i in range(2))
+            ref, tol = _attend64(q[b, h:h + 1], k, v, j[-1:], j, torch.ones(1, n, dtype=torch.bool, device=dev), 0.125, 0.0,
+                                 None, torch.float16)
+            _close(out[b, h:h + 1], ref, tol, f"sequence {b} head {h}")
+
+
+@pytest.mark.parametrize("hq,hkv,D", [(16, 4, 128), (8, 8, 64), (80, 4, 128)])
+def test_paged_heads_side_by_side(dev, hq, hkv, D):
+    """Enough work that four heads are read together, sequences of all lengths, with and without a window."""
+    lens = [4100, 1, 0, 2049, 3333, 16, 4096, 31, 1000, 2500] * 4
+    for window in (0, 700):
+        kv, table, ks, vs = _cache(dev, lens, 16, hkv, D, torch.bfloat16, 70)
+        q = torch.randn(len(lens), hq, D, generator=_gen(71), device=dev).bfloat16()
+        sl = torch.tensor(lens, device=dev)
+        out = S.compute_paged_attention(q, kv[0], kv[1], table, sl, max(lens), window=window, score_cap=40.0)
+        for b, n in enumerate(lens):
+            lo = max(0, n - window) if window else 0
+            j = torch.arange(lo, n, device=dev)
+            for h in (0, hq // 2, hq - 1) if n else ():
+                kh = h * hkv // hq
+                ref, tol = _attend64(q[b, h:h + 1], ks[b][lo:, kh], vs[b][lo:, kh], j[-1:], j,
+                                     torch.ones(1, n - lo, dtype=torch.bool, device=dev), 1 / math.sqrt(D), 40.0, None,
+                                     torch.bfloat16)
+                _close(out[b, h:h + 1], ref, tol, f"sequence {b} head {h}")
+            if n == 0:
+                assert bool((out[b] == 0).all())
+
+
+def test_paged_scores_that_are_not_finite(dev):
+    """A NaN key in one share makes its rows NaN, scores of -inf count for nothing beside finite ones, alone they are
+    NaN; other sequences and heads keep their bits."""
+    lens = [3000, 2000, 500]
+    kv, table, ks, vs = _cache(dev, lens, 16, 2, 64, torch.float16, 72)
+    q = torch.rand(3, 4, 64, generator=_gen(73), device=dev).half() + 0.1
+    sl = torch.tensor(lens, device=dev)
+    clean = S.compute_paged_attention(q, kv[0], kv[1], table, sl, 3000)
+    page = int(table[0, 100])
+    for bad, rows_nan in ((float("nan"), True), (-INF, False)):
+        x = kv.clone()
+        x[0, page, 3, 1] = bad
+        got = S.compute_paged_attention(q, x[0], x[1], table, sl, 3000)
+        assert torch.equal(got[1:], clean[1:]) and torch.equal(got[0, :2], clean[0, :2])
+        assert bool(torch.isnan(got[0, 2:]).all()) == rows_nan and bool(torch.isfinite(got[0, 2:]).all()) != rows_nan
+    x = kv.clone()
+    x[0][:, :, 1] = -INF
+    got = S.compute_paged_attention(q, x[0], x[1], table, sl, 3000)
+    assert bool(torch.isnan(got[:, 2:]).all()) and torch.equal(got[:, :2], clean[:, :2])
+    x = kv.clone()
+    x[1, page, 3, 1, 5] = float("nan")
+    got = S.compute_paged_attention(q, x[0], x[1], table, sl, 3000)
+    hit = torch.zeros_like(got, dtype=torch.bool)
+    hit[0, 2:, 5] = True
+    assert bool(torch.isnan(got[hit]).all()) and torch.equal(got[~hit], clean[~hit])
 
 
 def test_paged_bad_pages_and_empty_sequences(dev):
