@@ -42,11 +42,18 @@ def _slopes(what: str, alibi_slopes: Optional[torch.Tensor], heads: int):
     return (alibi_slopes if alibi_slopes.dtype == torch.float32 else alibi_slopes.float()).contiguous()
 
 
+def _int32(t: torch.Tensor) -> torch.Tensor:
+    """int32 or int64 as contiguous int32; numbers beyond it stay beyond any size."""
+    if t.dtype != torch.int32:
+        t = t.clamp(-(2 ** 31), 2 ** 31 - 1).to(torch.int32)
+    return t.contiguous()
+
+
 def _ints(what: str, name: str, t: torch.Tensor, n: int) -> torch.Tensor:
     """t [n] of integers as contiguous int32."""
     if t.dim() != 1 or t.shape[0] != n or t.dtype not in _INTEGERS:
         raise ValueError(f"{what}: {name} must be int32 or int64 [{n}], got {tuple(t.shape)} {t.dtype}")
-    return (t if t.dtype == torch.int32 else t.to(torch.int32)).contiguous()
+    return _int32(t)
 
 
 def _rows(t: torch.Tensor):
@@ -174,7 +181,7 @@ def compute_paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     slopes = _slopes(what, alibi_slopes, Hq)
     res = _out(what, out, q, k_cache, v_cache)
     q, (qb, qh) = _rows(q)
-    table = (block_table if block_table.dtype == torch.int32 else block_table.to(torch.int32)).contiguous()
+    table = _int32(block_table)
     lens = seq_lens.contiguous()
     p = _native.PagedParams(
         _TYPES[q.dtype], B, Hq, Hkv, D, bs, blocks, table.shape[1], window, lens.dtype == torch.int64, int(max_seq_len),

@@ -118,6 +118,18 @@ def test_norm_rotary_reads_views_in_place(dev):
     _check_rotary(a, x.view(10, 3, 64)[:3], p4.view(-1)[:3], rot, None)
 
 
+@pytest.mark.parametrize("dtype,interleaved", [(torch.bfloat16, False), (torch.float16, True), (torch.float32, False)])
+def test_norm_rotary_of_a_long_prompt(dev, dtype, interleaved):
+    """Results beyond what the caches hold take another kind of store."""
+    T = 7001 if dtype == torch.float32 else 14001
+    x = torch.randn(T, 20, 128, generator=_gen(8), device=dev).to(dtype)
+    rot, pos = S.RotaryPositions(64, interleaved=interleaved), torch.arange(T, device=dev)
+    w = torch.rand(128, generator=_gen(9), device=dev).to(dtype)
+    a, b = S.apply_norm_rotary(x, x[:, :3], pos, rot, w, w)
+    _check_rotary(a, x, pos, rot, w)
+    _check_rotary(b, x[:, :3], pos, rot, w)
+
+
 def test_norm_rotary_keeps_nonfinite_values_in_their_row(dev):
     g = _gen(7)
     rot = S.RotaryPositions(128)
@@ -426,6 +438,23 @@ def test_packed_infinite_scores(dev):
     assert bool((capped == 1).all())
 
 
+def test_packed_and_rotary_offsets_beyond_32_bits(dev):
+    """Rows that lie more than 2^31 elements into a packed projection."""
+    T, hq, hkv, D, doc = 360000, 32, 8, 128, 48
+    assert T * (hq + 2 * hkv) * D > 2 ** 31
+    x = torch.empty(T, hq + 2 * hkv, D, dtype=torch.bfloat16, device=dev)
+    x[:doc] = torch.randn(doc, hq + 2 * hkv, D, generator=_gen(28), device=dev)
+    for i in range(doc, T, doc * 100):   # every document is the first one
+        m = min(doc * 100, T - i)
+        x[i:i + m] = x[:doc].repeat(100, 1, 1)[:m]
+    starts = torch.arange(0, T + 1, doc, dtype=torch.int32, device=dev)
+    out = S.compute_packed_attention(x[:, :hq], x[:, hq:hq + hkv], x[:, hq + hkv:], starts)
+    assert bool(torch.isfinite(out[:doc]).all())
+    q, k = S.apply_norm_rotary(x[:, :hq], x[:, hq:hq + hkv], torch.arange(T, device=dev) % doc, S.RotaryPositions(D))
+    for t in (out, q, k):
+        assert torch.equal(t.view(T // doc, doc, -1), t[:doc].reshape(1, doc, -1).expand(T // doc, -1, -1))
+
+
 def test_packed_strides_and_alignment(dev):
     """Transposed, expanded and misaligned inputs give what contiguous ones give."""
     q, k, v = (t.contiguous() for t in _qkv(dev, 150, 4, 2, 64, torch.float16, 9))
@@ -608,6 +637,9 @@ def test_paged_bad_pages_and_empty_sequences(dev):
                              torch.ones(1, len(j), dtype=torch.bool, device=dev), 0.125, 0.0, None, torch.float16)
         _close(out[0, h:h + 1], ref, tol, f"head {h}")
     lens[3] = 10 ** 6                                     # 9 table entries, the last -1: 16 tokens are there
+    wide = table.long()
+    wide[0, 2], wide[0, 5], wide[1, :] = 2 ** 32, 2 ** 32 + 1, -(2 ** 40)       # no wrapping into the cache either
+    assert torch.equal(S.compute_paged_attention(q, kv[0], kv[1], wide, lens.clamp(max=100), 100)[:3], out[:3])
     long = S.compute_paged_attention(q, kv[0], kv[1], table, lens, 10 ** 6)
     ok = S.compute_paged_attention(q, kv[0], kv[1], table, torch.tensor([100, 64, -5, 16], device=dev), 100)
     _close(long[3], ok[3].double(), 2 ** -10 * ok[3].double().abs() + 2 ** -10 * vs[3].abs().max().double(), "cut")
