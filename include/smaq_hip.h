@@ -474,8 +474,8 @@ typedef struct smaq_packed_params {
   int window;                /* 0: none */
   int zero_rest;             /* rows of no document: 1 written as zeros, 0 left as they are */
   long long n_tokens;        /* rows of q, k, v and out */
-  float scale;
-  float score_cap;           /* 0: none */
+  float scale;               /* below 1e38 */
+  float score_cap;           /* 0: none; else 1e-30..1e30 */
   const int* starts;         /* [n_docs + 1], ascending (numbers outside 0..n_tokens are cut) */
   const int* prefix_lens;    /* [n_docs] or NULL */
   const float* alibi_slopes; /* [n_q_heads] or NULL */
@@ -508,8 +508,8 @@ typedef struct smaq_paged_params {
   int window;                /* 0: none */
   int seq_lens_wide;         /* seq_lens is int64, else int32 */
   long long max_seq_len;     /* no sequence is longer */
-  float scale;
-  float score_cap;           /* 0: none */
+  float scale;               /* below 1e38 */
+  float score_cap;           /* 0: none; else 1e-30..1e30 */
   const void* seq_lens;      /* [batch] */
   const int* block_table;    /* [batch][max_blocks] */
   const float* alibi_slopes; /* [n_q_heads] or NULL */

@@ -1,6 +1,8 @@
 // What the two attention kernels over exact keys share (not part of the C ABI).
 #pragma once
 
+#include <math.h>
+
 #include "smaq_common.h"
 
 namespace smaq {
@@ -26,9 +28,17 @@ inline bool rows_on_16(const void* p, S... strides) {
   return (uintptr_t)p % 16 == 0 && ((strides % 8 == 0) && ...);
 }
 
+// Whether the fp32 forms below hold: no scale or cap that leaves the range.
+inline bool score_range(float scale, float cap) {
+  return fabsf(scale) < 1e38f && (cap == 0.0f || (cap >= 1e-30f && cap < 1e30f));
+}
+
 inline ScoreRule score_rule(float scale, float cap) {
-  if (cap > 0.0f)
-    return {(float)(2.0 * 1.4426950408889634 * (double)scale / (double)cap), cap * kLog2eF, cap > kWideCap};
+  if (cap > 0.0f) {
+    // finite, so that a product of 0 has the score 0
+    const double x = 2.0 * 1.4426950408889634 * (double)scale / (double)cap;
+    return {(float)fmin(fmax(x, -3e38), 3e38), cap * kLog2eF, cap > kWideCap};
+  }
   return {scale * kLog2eF, 0.0f, 0};
 }
 

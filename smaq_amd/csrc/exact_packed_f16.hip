@@ -17,9 +17,9 @@ extern "C" int smaq_packed_attention(const smaq_packed_params* p, void* stream) 
                p->n_q_heads, p->n_kv_heads);
   SMAQ_REQUIRE(p->head_dim > 0 && p->head_dim <= 256 && p->head_dim % 8 == 0,
                "smaq_packed_attention: head_dim %d is not a multiple of 8 up to 256", p->head_dim);
-  SMAQ_REQUIRE(p->window >= 0 && p->score_cap >= 0.0f && p->score_cap < 1e30f && p->scale == p->scale,
-               "smaq_packed_attention: window %d, score_cap %g and scale %g must be numbers of 0 or more, finite and "
-               "a number", p->window, (double)p->score_cap, (double)p->scale);
+  SMAQ_REQUIRE(p->window >= 0 && score_range(p->scale, p->score_cap),
+               "smaq_packed_attention: window %d must be 0 or more, score_cap %g 0 or in 1e-30..1e30, scale %g below 1e38",
+               p->window, (double)p->score_cap, (double)p->scale);
   if (p->dtype != SMAQ_F16 && p->dtype != SMAQ_BF16) {
     set_error("smaq_packed_attention: unsupported dtype %d", p->dtype);
     return SMAQ_EUNSUPPORTED;

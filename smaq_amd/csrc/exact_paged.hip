@@ -519,9 +519,9 @@ int check_paged(const smaq_paged_params* p) {
                    p->max_blocks >= 0 && p->max_seq_len >= 0,
                "smaq_paged_attention: block_size %d must be a multiple of 16 (num_blocks %d, max_blocks %d, max_seq_len "
                "%lld of 0 or more)", p->block_size, p->num_blocks, p->max_blocks, p->max_seq_len);
-  SMAQ_REQUIRE(p->window >= 0 && p->score_cap >= 0.0f && p->score_cap < 1e30f && p->scale == p->scale,
-               "smaq_paged_attention: window %d, score_cap %g and scale %g must be numbers of 0 or more, finite and a "
-               "number", p->window, (double)p->score_cap, (double)p->scale);
+  SMAQ_REQUIRE(p->window >= 0 && score_range(p->scale, p->score_cap),
+               "smaq_paged_attention: window %d must be 0 or more, score_cap %g 0 or in 1e-30..1e30, scale %g below 1e38",
+               p->window, (double)p->score_cap, (double)p->scale);
   if (p->dtype != SMAQ_F16 && p->dtype != SMAQ_BF16) {
     set_error("smaq_paged_attention: unsupported dtype %d", p->dtype);
     return SMAQ_EUNSUPPORTED;

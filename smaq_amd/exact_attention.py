@@ -24,10 +24,10 @@ _TYPES = {torch.float16: _native.F16, torch.bfloat16: _native.BF16}
 
 def _scores(what: str, head_dim: int, scale: Optional[float], score_cap: float, window: int):
     scale = 1.0 / math.sqrt(head_dim) if scale is None else float(scale)
-    if not math.isfinite(scale):
-        raise ValueError(f"{what}: scale must be finite, got {scale}")
-    if not (0.0 <= score_cap < 1e30):
-        raise ValueError(f"{what}: score_cap must be 0 (none) or a finite number above it, got {score_cap}")
+    if not abs(scale) < 1e38:
+        raise ValueError(f"{what}: scale must be a number below 1e38, got {scale}")
+    if score_cap != 0.0 and not 1e-30 <= score_cap < 1e30:
+        raise ValueError(f"{what}: score_cap must be 0 (none) or a number from 1e-30 to 1e30, got {score_cap}")
     if window < 0 or window > 0x7fffffff:
         raise ValueError(f"{what}: window must be 0 (none) or a number of tokens, got {window}")
     return scale, float(score_cap), int(window)
@@ -184,7 +184,8 @@ def compute_paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     table = _int32(block_table)
     lens = seq_lens.contiguous()
     p = _native.PagedParams(
-        _TYPES[q.dtype], B, Hq, Hkv, D, bs, blocks, table.shape[1], window, lens.dtype == torch.int64, int(max_seq_len),
+        _TYPES[q.dtype], B, Hq, Hkv, D, bs, blocks, table.shape[1], window, lens.dtype == torch.int64,
+        min(int(max_seq_len), 0x7fffffff),
         scale, cap, lens.data_ptr(), table.data_ptr(), None if slopes is None else slopes.data_ptr(), q.data_ptr(),
         k_cache.data_ptr(), v_cache.data_ptr(), res.data_ptr(), qb, qh, Hq * D, D, *k_steps, *v_steps)
     lib, ref = _native.lib(), ctypes.byref(p)

@@ -60,9 +60,10 @@ def build_page_step(context_lens: torch.Tensor, new_lens: torch.Tensor, block_ta
         start = t.data_ptr()
         if start < end and start + t.shape[0] * t.element_size() > table:
             raise ValueError(f"build_page_step: block_table shares memory with {what}")
-    num_tokens = int(num_tokens)
-    if num_tokens < 0:
-        raise ValueError(f"build_page_step: num_tokens must be 0 or more, got {num_tokens}")
+    num_tokens, block_size = int(num_tokens), int(block_size)
+    if not (0 <= num_tokens <= 0x7fffffff and 1 <= block_size <= 65536):
+        raise ValueError(f"build_page_step: num_tokens must be 0 or more, got {num_tokens}, and block_size 1..65536, got "
+                         f"{block_size}")
     dev = block_table.device
     slots = torch.empty(num_tokens, dtype=torch.int64, device=dev)
     positions = torch.empty(num_tokens, dtype=torch.int64, device=dev)
@@ -71,6 +72,6 @@ def build_page_step(context_lens: torch.Tensor, new_lens: torch.Tensor, block_ta
     status = torch.empty(2, dtype=torch.int32, device=dev)
     _native.launch_on(index, _native.lib().smaq_page_step, "smaq_page_step", ctx.data_ptr(), ctx.element_size(),
                       new.data_ptr(), new.element_size(), n, table, width, free.data_ptr(), free.shape[0],
-                      int(block_size), num_tokens, slots.data_ptr(), positions.data_ptr(), starts.data_ptr(),
+                      block_size, num_tokens, slots.data_ptr(), positions.data_ptr(), starts.data_ptr(),
                       seq_lens.data_ptr(), status.data_ptr())
     return PageStep(slots, positions, starts, seq_lens, status)

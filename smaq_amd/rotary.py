@@ -67,8 +67,8 @@ class RotaryPositions:
                 self.gain = 0.1 * math.log(factor) + 1.0
         if attention_factor is not None:
             self.gain = float(attention_factor)
-        if not bool(torch.isfinite(table).all()) or not math.isfinite(self.gain):
-            raise ValueError("frequencies and attention_factor must be finite")
+        if not bool(torch.isfinite(table).all()) or not abs(self.gain) < 1e38:
+            raise ValueError("frequencies must be finite, attention_factor a number below 1e38")
         self.freqs = table.contiguous().to(device)
 
     def _schedule(self, half, base, scaling, factor, original_length, beta_fast, beta_slow) -> torch.Tensor:
@@ -138,8 +138,8 @@ def apply_norm_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: tor
             if w.dim() != 1 or w.shape[0] != D or w.dtype != weight_dtype:
                 raise ValueError(f"apply_norm_rotary: weights must be [{D}] and of one dtype, got {tuple(w.shape)} "
                                  f"{w.dtype}")
-    if not (0.0 <= eps < math.inf and math.isfinite(weight_offset)):
-        raise ValueError("apply_norm_rotary: eps must be a finite number of 0 or more, weight_offset finite")
+    if not (0.0 <= eps < 1e38 and abs(weight_offset) < 1e38):
+        raise ValueError("apply_norm_rotary: eps must be a number from 0 to 1e38, weight_offset one below 1e38")
     code = _native.dtype_code(dtype)
     weight_code = _native.F32 if weight_dtype is None else _native.dtype_code(weight_dtype)
     qf = _heads("queries", q, lead, D, dtype)

@@ -244,3 +244,33 @@ def test_c_entries_refuse_before_any_launch():
     g.q = g.out = g.seq_lens = g.block_table = g.k_cache = g.v_cache = d
     g.k_stride_t = 4
     assert lib.smaq_paged_attention(ctypes.byref(g), None) == -1 and b"16 bytes" in lib.smaq_last_error()
+
+
+@pytest.mark.parametrize("kw", [dict(scale=1e39), dict(scale=-1e38), dict(score_cap=1e-50), dict(score_cap=1e30)])
+def test_scales_and_caps_beyond_fp32_are_refused(no_gpu_check, kw):
+    with pytest.raises(ValueError, match="scale|score_cap"):
+        S.compute_packed_attention(**_packed_args(**kw))
+    with pytest.raises(ValueError, match="scale|score_cap"):
+        S.compute_paged_attention(**_paged_args(**kw))
+    k, g = _native.PackedParams(), _native.PagedParams()
+    for p, fn in ((k, "smaq_packed_attention"), (g, "smaq_paged_attention")):
+        p.dtype, p.n_q_heads, p.n_kv_heads, p.head_dim = 1, 2, 2, 64
+        p.scale, p.score_cap = kw.get("scale", 1.0), kw.get("score_cap", 0.0)
+        if p is g:
+            p.block_size = 16
+        if kw.get("score_cap") != 1e-50:  # which a float argument turns into none
+            assert getattr(_native.lib(), fn)(ctypes.byref(p), None) == -1 and b"scale" in _native.lib().smaq_last_error()
+
+
+@pytest.mark.parametrize("kw", [dict(eps=1e39), dict(weight_offset=-1e39)])
+def test_norm_constants_beyond_fp32_are_refused(no_gpu_check, kw):
+    with pytest.raises(ValueError):
+        S.apply_norm_rotary(**_rotary_args(**kw))
+    with pytest.raises(ValueError):
+        S.RotaryPositions(64, attention_factor=1e39, device="cpu")
+
+
+@pytest.mark.parametrize("kw", [dict(block_size=0), dict(block_size=2 ** 32 + 16), dict(num_tokens=2 ** 31)])
+def test_page_sizes_beyond_an_int_are_refused(no_gpu_check, kw):
+    with pytest.raises(ValueError, match="block_size"):
+        S.build_page_step(**_page_args(**kw))

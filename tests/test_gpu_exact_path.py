@@ -798,3 +798,52 @@ def test_gradients_are_refused(dev):
         S.compute_packed_attention(q, k.clone().requires_grad_(), v, starts)
     with torch.no_grad():
         S.compute_packed_attention(q, k.clone().requires_grad_(), v, starts)
+
+
+def test_two_calls_at_once(dev):
+    """Two streams run the same operators on their own inputs side by side: each gets what it gets alone."""
+    kv, table, _, _ = _cache(dev, [4000, 7, 2500], 16, 4, 128, torch.bfloat16, 40)
+    rot = S.RotaryPositions(128)
+    starts, pos = _starts([700, 333], dev), torch.arange(1033, device=dev)
+    qkv = [_qkv(dev, 1033, 8, 4, 128, torch.bfloat16, 41 + i) for i in range(2)]
+    lens = [torch.tensor(x, dtype=torch.int32, device=dev) for x in ([4000, 7, 2500], [1999, 0, 2500])]
+    ctx = [torch.tensor(x, dtype=torch.int32, device=dev) for x in ([17, 3, 16], [0, 31, 5])]
+    tables = [torch.zeros(3, 8, dtype=torch.int32, device=dev) for _ in range(2)]
+    new, free = torch.full((3,), 20, dtype=torch.int32, device=dev), torch.arange(100, 120, dtype=torch.int32, device=dev)
+
+    def both(i):
+        q, k, v = qkv[i]
+        a, b = S.apply_norm_rotary(q, k, pos, rot)
+        return (a, b, S.compute_packed_attention(a, b, v, starts, score_cap=20.0),
+                S.compute_paged_attention(a[:3], kv[0], kv[1], table, lens[i], 4000),
+                *S.build_page_step(ctx[i], new, tables[i], free, 16, 64), tables[i].clone())
+    want = [both(0), both(1)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(both(i))
+    for s in streams:
+        torch.cuda.current_stream().wait_stream(s)
+    for i in range(2):
+        for outs in got[i]:
+            assert all(torch.equal(x, y) for x, y in zip(outs, want[i]))
+
+
+@pytest.mark.parametrize("kw", [dict(score_cap=1e-20, scale=1e30), dict(score_cap=1e-30), dict(score_cap=9e29)])
+def test_caps_at_the_ends_of_their_range(dev, kw):
+    """Queries of 0 score 0 under any cap: the mean of the values, each weight exact, half a step of rounding."""
+    q, k, v = (torch.randn(64, 2, 64, generator=_gen(44), device=dev).half() for _ in range(3))
+    q.zero_()
+    kv = torch.stack([k, v]).view(2, 4, 16, 2, 64)
+    packed = S.compute_packed_attention(q, k, v, _starts([64], dev), causal=False, **kw)
+    paged = S.compute_paged_attention(q[:1], kv[0], kv[1], torch.arange(4, dtype=torch.int32, device=dev)[None],
+                                      torch.tensor([64], device=dev), 64, **kw)
+    ref = v.double().mean(0)
+    # sums of 64 products of at most max|v| in fp32, then one rounding
+    tol = 2.0 ** -11 * ref.abs() + 64 * 2.0 ** -24 * v.double().abs().amax() + 2.0 ** -25
+    for out in (*packed, paged[0]):
+        _close(out, ref, tol, str(kw))
