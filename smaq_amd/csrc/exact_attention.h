@@ -15,12 +15,19 @@ struct ScoreRule {
   float scale;  // no cap: scale log2(e); cap: 2 log2(e) scale / cap
   float cap;    // cap log2(e); 0: none
   int wide;     // the cap is above kWideCap
+  float near;   // products below this in size may take near_score; 0: none
+  float c[4];   // of near_score
 };
 
 // cap (1 - 2 / (e^(2x/cap) + 1)) loses what lies below some 2^-22 of the cap: up to
 // this cap that moves a weight by less than 2^-13 (half a step of fp16 is 2^-11);
 // above it small arguments take the series of tanh.
 constexpr float kWideCap = 256.0f;
+
+// tanh(y) / y as a polynomial in y^2: interpolated at Chebyshev's points for |y| <= kNearTanh,
+// off by 2^-20.8 of the value at most, half a cap's 2^-21.
+constexpr double kNearTanh = 0.5;
+constexpr double kTanh[4] = {0.99999945, -0.33326284, 0.13189939, -0.04439274};
 
 // Whether rows of 16-bit elements start on 16 bytes.
 template <typename... S>
@@ -37,9 +44,18 @@ inline ScoreRule score_rule(float scale, float cap) {
   if (cap > 0.0f) {
     // finite, so that a product of 0 has the score 0
     const double x = 2.0 * 1.4426950408889634 * (double)scale / (double)cap;
-    return {(float)fmin(fmax(x, -3e38), 3e38), cap * kLog2eF, cap > kWideCap};
+    ScoreRule r{(float)fmin(fmax(x, -3e38), 3e38), cap * kLog2eF, cap > kWideCap, 0.0f, {}};
+    const double a = fabs((double)scale) / (double)cap, near = kNearTanh / a;
+    bool fits = cap <= kWideCap && near > 1e-15 && near < 1e15;
+    double f = 1.4426950408889634 * (double)scale;  // cap log2(e) a^(2k + 1)
+    for (int k = 0; k < 4; ++k, f *= a * a) {
+      r.c[k] = (float)(f * kTanh[k]);
+      fits = fits && fabsf(r.c[k]) > 1e-37f && fabsf(r.c[k]) < 1e37f;
+    }
+    if (fits) r.near = (float)near;
+    return r;
   }
-  return {scale * kLog2eF, 0.0f, 0};
+  return {scale * kLog2eF, 0.0f, 0, 0.0f, {}};
 }
 
 // cap tanh(x / cap) of x = scale dot, times log2(e).  The limits at +-inf are exact,
@@ -53,6 +69,12 @@ __device__ __forceinline__ float capped_score(const ScoreRule& r, float dot) {
   const float y = x * (0.5f / kLog2eF), z = y * y;
   const float s = fmaf(z, fmaf(z, fmaf(z, 62.0f / 2835.0f, -17.0f / 315.0f), 2.0f / 15.0f), -1.0f / 3.0f);
   return fabsf(y) < 0.35f ? r.cap * fmaf(y * z, s, y) : t;
+}
+
+// The same for |dot| < near, with no exponential or reciprocal.
+__device__ __forceinline__ float near_score(const ScoreRule& r, float dot, float less = 0.0f) {
+  const float z = dot * dot;
+  return fmaf(dot, fmaf(z, fmaf(z, fmaf(z, r.c[3], r.c[2]), r.c[1]), r.c[0]), -less);
 }
 
 // put(i, score of the product get(i)) for N products: one uniform choice of the rule

@@ -222,19 +222,33 @@ __global__ __launch_bounds__(KG * kThreads, DT == 64 && KG == 1 ? 3 : 2) void pa
   const T* kc = (const T*)p.k + h * p.k_stride_h;
   const T* vc = (const T*)p.v + h * p.v_stride_h;
   const int r0 = tid / UPR, u0 = tid % UPR;
+  constexpr int PER = RPL < 16 ? 2 : 1;  // loads until the swizzle of a row returns
+  static_assert(RPL * PER % 16 == 0, "whole periods");
+  uint32_t k_lane[PER];
+  for (int i = 0; i < PER; ++i) k_lane[i] = (uint32_t)(2 * r0 * (int)p.k_stride_t) + 16 * (u0 ^ key_swizzle<DT>(i * RPL + r0));
+  const uint32_t v_lane = (uint32_t)(2 * r0 * (int)p.v_stride_t) + 16 * (u0 ^ val_swizzle<DT>(r0));
   auto to_lds = [&](const void* src, char* dst) {
     __builtin_amdgcn_global_load_lds(src, (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
   };
   auto copy_tile = [&](int k, int buf) {
     char* kd = lds + buf * 2 * TILE + 1024 * w;
     if (FULL && k + KT <= k_hi) {
-      // whole tiles: a base of the wave and a 32-bit offset of the lane
-      const uint32_t ko = (uint32_t)(2 * r0 * (int)p.k_stride_t), vo = (uint32_t)(2 * r0 * (int)p.v_stride_t);
+      // whole tiles: a base of the wave and a 32-bit offset of the lane (not hoisted as 64
+      // bits, which the load does not take as an offset)
+      uint32_t ko[PER], vo = v_lane;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        ko[i] = k_lane[i];
+        asm volatile("" : "+v"(ko[i]));
+      }
+      asm volatile("" : "+v"(vo));
+      const char *ks = (const char*)(kc + k * p.k_stride_t), *vs = (const char*)(vc + k * p.v_stride_t);
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
-        const int r = i * RPL + r0;
-        to_lds((const char*)(kc + (int64_t)(k + i * RPL) * p.k_stride_t) + (ko + 16 * (u0 ^ key_swizzle<DT>(r))), kd + 4096 * i);
-        to_lds((const char*)(vc + (int64_t)(k + i * RPL) * p.v_stride_t) + (vo + 16 * (u0 ^ val_swizzle<DT>(r))), kd + TILE + 4096 * i);
+        to_lds(ks + ko[i % PER], kd + 4096 * i);
+        to_lds(vs + vo, kd + TILE + 4096 * i);
+        ks += 2 * RPL * p.k_stride_t;
+        vs += 2 * RPL * p.v_stride_t;
       }
       return;
     }
@@ -286,18 +300,43 @@ __global__ __launch_bounds__(KG * kThreads, DT == 64 && KG == 1 ? 3 : 2) void pa
       if (k_mine < k_hi) copy_tile(k_mine, buf ^ 1);
       if (k0 >= w_hi || k0 + KT <= w_lo || (k0 >= w_gap0 && k0 + KT <= w_gap1)) continue;
       const int kt = buf * 2 * TILE + koff, vt = buf * 2 * TILE + TILE + voff;
-      f32x16v s[KB];
-      if constexpr (PRIO) __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb) {
-        s[kb] = f32x16v{};
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-          s[kb] = Mat<T>::mma32(*(const u32x4v*)(lds + (kt ^ (32 * ks)) + kb * 32 * RS), qr[ks], s[kb]);
-      }
-      if constexpr (PRIO) __builtin_amdgcn_s_setprio(0);
       // key of register i of block kb: k0 + 32 kb + 8 (i / 4) + 4 half + i % 4
       const bool full = k0 >= w_full0 && k0 + KT <= w_full1;
+      f32x16v s[KB];
+      // put(kb, i, whether the row sees the key)
+      auto each_seen = [&](auto put) {
+        const int a1 = hi - k0 - 4 * half;
+        if (!w_apart && k0 >= w_full0) {  // causal and last tiles: cut above only
+#pragma unroll
+          for (int i = 0; i < 16 * KB; ++i) put(i / 16, i % 16, 32 * (i / 16) + 8 * (i % 16 / 4) + i % 4 < a1);
+          return;
+        }
+        const int a0 = lo - k0 - 4 * half, b0 = lo2 - k0 - 4 * half, b1 = hi2 - k0 - 4 * half;
+#pragma unroll
+        for (int i = 0; i < 16 * KB; ++i) {
+          const int key = 32 * (i / 16) + 8 * (i % 16 / 4) + i % 4;
+          put(i / 16, i % 16, ((key >= a0) & (key < a1)) | ((key >= b0) & (key < b1)));
+        }
+      };
+      auto product = [&](auto masked_tag) {
+        if constexpr (PRIO) __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+          if constexpr (!decltype(masked_tag)::value) s[kb] = f32x16v{};
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks)
+            s[kb] = Mat<T>::mma32(*(const u32x4v*)(lds + (kt ^ (32 * ks)) + kb * 32 * RS), qr[ks], s[kb]);
+        }
+        if constexpr (PRIO) __builtin_amdgcn_s_setprio(0);
+      };
+      // A masked tile's sums begin at -inf where the key is not seen: code of its own, as
+      // masks behind one product cost whole tiles 16 register copies
+      if (full) {
+        product(std::false_type{});
+      } else {
+        each_seen([&](int kb, int i, bool seen) { s[kb][i] = seen ? 0.0f : kNegInf; });
+        product(std::true_type{});
+      }
       auto get = [&](int i) { return s[i / 16][i % 16]; };
       if constexpr (ALIBI) {
         const float gap = (float)(row - k0 - 4 * half);
@@ -311,30 +350,20 @@ __global__ __launch_bounds__(KG * kThreads, DT == 64 && KG == 1 ? 3 : 2) void pa
           for (int i = 0; i < 16 * KB; ++i) put(i, get(i) * rule.scale);
         }
       }
-      if (!full && !w_apart && k0 >= w_full0) {  // causal and last tiles: cut above only
-        const int a1 = hi - k0 - 4 * half;
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) s[kb][i] = 32 * kb + 8 * (i / 4) + i % 4 < a1 ? s[kb][i] : kNegInf;
-      } else if (!full) {
-        const int a0 = lo - k0 - 4 * half, a1 = hi - k0 - 4 * half, b0 = lo2 - k0 - 4 * half, b1 = hi2 - k0 - 4 * half;
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int key = 32 * kb + 8 * (i / 4) + i % 4;
-            const bool seen = ((key >= a0) & (key < a1)) | ((key >= b0) & (key < b1));
-            s[kb][i] = seen ? s[kb][i] : kNegInf;
-          }
-      }
-      float mx = kNegInf;
+      // -inf plus a product that is not finite, and -inf behind a cap, are no longer -inf
+      if (careful || (CAP && ALIBI))
+        if (!full) each_seen([&](int kb, int i, bool seen) { s[kb][i] = seen ? s[kb][i] : kNegInf; });
+      float mx = kNegInf, size = 0.0f;
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kb][i]);
+        for (int i = 0; i < 16; ++i) {
+          mx = fmaxf(mx, s[kb][i]);
+          if constexpr (CAP && !ALIBI) size = fmaxf(size, fabsf(s[kb][i]));
+        }
+      const bool near = CAP && !ALIBI && __all(size < rule.near);  // of the wave; never with a masked key
       if constexpr (CAP && !ALIBI)
-        mx = rule.wide ? capped_score<true>(rule, mx) : capped_score<false>(rule, mx);
+        mx = near ? near_score(rule, mx) : rule.wide ? capped_score<true>(rule, mx) : capped_score<false>(rule, mx);
       else if constexpr (!ALIBI)
         mx *= rule.scale;
       if (__any(mx > m_thr)) {
@@ -349,7 +378,12 @@ __global__ __launch_bounds__(KG * kThreads, DT == 64 && KG == 1 ? 3 : 2) void pa
         m_thr = m_new + kRaise;
       }
       if constexpr (CAP && !ALIBI) {
-        each_score<16 * KB>(rule, get, [&](int i, float x) { s[i / 16][i % 16] = __builtin_amdgcn_exp2f(x - m_use); });
+        if (near) {
+#pragma unroll
+          for (int i = 0; i < 16 * KB; ++i) s[i / 16][i % 16] = __builtin_amdgcn_exp2f(near_score(rule, get(i), m_use));
+        } else {
+          each_score<16 * KB>(rule, get, [&](int i, float x) { s[i / 16][i % 16] = __builtin_amdgcn_exp2f(x - m_use); });
+        }
       } else {
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
@@ -358,17 +392,7 @@ __global__ __launch_bounds__(KG * kThreads, DT == 64 && KG == 1 ? 3 : 2) void pa
             s[kb][i] = __builtin_amdgcn_exp2f(ALIBI ? s[kb][i] - m_use : fmaf(s[kb][i], rule.scale, -m_use));
       }
       if constexpr (CAP && !ALIBI) {  // the cap brings a masked score back to -cap
-        if (!full) {
-          const int a0 = lo - k0 - 4 * half, a1 = hi - k0 - 4 * half, b0 = lo2 - k0 - 4 * half, b1 = hi2 - k0 - 4 * half;
-#pragma unroll
-          for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const int key = 32 * kb + 8 * (i / 4) + i % 4;
-              const bool seen = ((key >= a0) & (key < a1)) | ((key >= b0) & (key < b1));
-              s[kb][i] = seen ? s[kb][i] : 0.0f;
-            }
-        }
+        if (!full) each_seen([&](int kb, int i, bool seen) { s[kb][i] = seen ? s[kb][i] : 0.0f; });
       }
       uint32_t pk[KB][8];
 #pragma unroll
