@@ -22,6 +22,12 @@
 // head in turn, or four heads side by side (HW = 4): rows of four heads lie next to each
 // other, and reading them together is kinder to the memory.
 //
+// 32 sequences of 32768 tokens, 32 / 8 heads of 128 bf16 dims (4.3 GB): 0.72 ms, 6.0 TB/s;
+// 256 of 1 to 4096 tokens, capped (1.5 GB): 0.27 ms, 5.5 TB/s, 13 us of it the merge; one of
+// 65408 tokens (134 MB): 34 us, 3.9 TB/s, 6 us of it the merge.  A plain read of that size
+// reaches 7.2 TB/s, a copy 5.2.  Weights are rounded to the values' type for the second
+// product, as the matrix instruction takes two operands of one type; all else is fp32.
+//
 // All steps of the batch are dealt to the workgroups in equal shares, however long
 // each sequence is: a share begins and ends inside sequences, and a row whose steps
 // went to several workgroups is joined from their partial results in order by a second

@@ -847,3 +847,21 @@ def test_caps_at_the_ends_of_their_range(dev, kw):
     tol = 2.0 ** -11 * ref.abs() + 64 * 2.0 ** -24 * v.double().abs().amax() + 2.0 ** -25
     for out in (*packed, paged[0]):
         _close(out, ref, tol, str(kw))
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("kw", [dict(score_cap=50.0), dict(score_cap=2.0), dict(slopes=True),
+                                dict(score_cap=20.0, slopes=True), dict(window=33, score_cap=50.0)])
+def test_packed_unseen_places_under_caps_and_biases(dev, kw, D):
+    """NaN, infinities and numbers whose products overflow above a row and in other documents leave its bits."""
+    kw, lens, at = dict(kw), [70, 300, 90], 70 + 171
+    if kw.pop("slopes", False):
+        kw["alibi_slopes"] = torch.tensor([0.5, 0.01], device=dev)
+    q, k, v = _qkv(dev, 460, 2, 1, D, torch.bfloat16, 46)
+    clean = S.compute_packed_attention(q, k, v, _starts(lens, dev), **kw)
+    for bad in (float("nan"), INF, -INF, 3e38):
+        for which in "kv":
+            x = {"k": k.clone(), "v": v.clone()}
+            x[which][at:370] = bad
+            got = S.compute_packed_attention(q, x["k"], x["v"], _starts(lens, dev), **kw)
+            assert torch.equal(got[:at], clean[:at]) and torch.equal(got[370:], clean[370:]), (bad, which)
