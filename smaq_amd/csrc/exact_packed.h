@@ -5,7 +5,7 @@
 // cores bound it, and beside them the power they share with the vector unit (the
 // exponentials) and LDS (operand reads): the clock falls from 2.4 to 1.7-1.9 GHz.
 // 16384 causal tokens of 32 / 8 heads of 128 bf16 dims take 2.1 ms (1.04 PFLOP/s; a 16384^3
-// matrix product reaches 1.58), capped 2.6 ms (0.85), biased 2.4 (0.91).  A tile less
+// matrix product reaches 1.58), capped 2.5 ms (0.87), biased 2.4 (0.91).  A tile less
 // vector work moves that little: without the exponentials it is 4% shorter, without the
 // copies to LDS 15%; eight waves on one copy, with two or three buffers, take 1-4% longer
 // than two workgroups of four, tiles of 32 keys 3%.
@@ -99,10 +99,10 @@ __global__ __launch_bounds__(KG * kThreads, DT == 64 && KG == 1 ? 3 : 2) void pa
   constexpr int RS = DT * 2;               // bytes of a row
   constexpr int TILE = KT * RS;            // bytes of a key or value tile
   constexpr int LOADS = KT * UPR / kThreads;
-  // Matrix sections at raised wave priority: 16384 capped tokens 2.69 -> 2.64 ms, 256 dims
-  // 1.17 -> 1.12 ms; without a cap at up to 128 dims they are better left alone (2.14 -> 2.11
-  // ms, 8192 tokens of 8 / 8 heads 231 -> 214 us).
-  constexpr bool PRIO = CAP || DT == 256;
+  // Matrix sections at raised wave priority: 256 dims 1.17 -> 1.12 ms; at up to 128 dims they
+  // are better left alone (16384 tokens 2.14 -> 2.11 ms, capped 2.56 -> 2.53, 8192 tokens of
+  // 8 / 8 heads 231 -> 214 us).
+  constexpr bool PRIO = DT == 256;
   __shared__ __attribute__((aligned(16))) char all_lds[KG * 4 * TILE];  // of each key group two buffers of (keys, values)
   __shared__ int span[4][4];
   __shared__ float joined[KG == 2 ? 4 : 1][2][64];
