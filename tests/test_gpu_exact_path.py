@@ -865,3 +865,47 @@ def test_packed_unseen_places_under_caps_and_biases(dev, kw, D):
             x[which][at:370] = bad
             got = S.compute_packed_attention(q, x["k"], x["v"], _starts(lens, dev), **kw)
             assert torch.equal(got[:at], clean[:at]) and torch.equal(got[370:], clean[370:]), (bad, which)
+
+
+@pytest.mark.parametrize("n", [65535, 1000003])
+def test_very_many_documents_of_one_token(dev, n):
+    """A token that sees itself alone has its value, bit for bit."""
+    q, k, v = _qkv(dev, n, 2, 1, 8, torch.float16, 48)
+    out = S.compute_packed_attention(q, k, v, torch.arange(n + 1, device=dev), score_cap=30.0)
+    assert torch.equal(out, v.expand(-1, 2, -1))
+
+
+@pytest.mark.parametrize("longest", [16, 400])
+def test_the_most_sequences(dev, longest):
+    """65535 sequences, most of them empty or of one token; the rest see equal keys, and so the mean of their values."""
+    n, d = 65535, 8
+    lens = torch.ones(n, dtype=torch.int32, device=dev)
+    lens[::7] = 0
+    lens[5::9973] = longest
+    kv = torch.zeros(2, 40, 16, 1, d, dtype=torch.float16, device=dev)
+    kv[1] = torch.randn(40, 16, 1, d, generator=_gen(49), device=dev).half()
+    table = torch.randint(0, 40, (n, (longest + 15) // 16), generator=_gen(50), device=dev)
+    q = torch.randn(n, 2, d, generator=_gen(51), device=dev).half()
+    out = S.compute_paged_attention(q, kv[0], kv[1], table, lens, longest)
+    first = kv[1][table[:, 0], 0, 0]
+    assert bool((out[lens == 0] == 0).all())
+    one = lens == 1
+    assert torch.equal(out[one], first[one][:, None].expand(-1, 2, -1))
+    for b in torch.nonzero(lens == longest).flatten().tolist():
+        seen = kv[1][table[b]].reshape(-1, d)[:longest].double()
+        ref = seen.mean(0)
+        # weights of 1; a sum of `longest` values in fp32, one rounding
+        tol = 2.0 ** -11 * ref.abs() + longest * 2.0 ** -24 * seen.abs().amax() + 2.0 ** -25
+        _close(out[b], ref.expand(2, -1), tol.expand(2, -1), f"sequence {b}")
+
+
+def test_the_largest_page_step(dev):
+    """8000 requests with long contexts and the longest blocks: slots beyond 32 bits."""
+    n, bs = 8000, 65536
+    ctx = torch.full((n,), 70000, dtype=torch.int64, device=dev)
+    new = torch.full((n,), 3, dtype=torch.int32, device=dev)
+    table = torch.full((n, 2), 2 ** 31 - 1, dtype=torch.int32, device=dev)
+    step = S.build_page_step(ctx, new, table, torch.empty(0, dtype=torch.int32, device=dev), bs, 3 * n)
+    want = (2 ** 31 - 1) * bs + 70000 - bs
+    assert step.slot_mapping.view(n, 3).tolist() == [[want, want + 1, want + 2]] * n
+    assert step.status.tolist() == [0, 0] and int(step.query_start_loc[-1]) == 3 * n
