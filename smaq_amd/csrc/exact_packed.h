@@ -226,6 +226,9 @@ __global__ __launch_bounds__(KG * kThreads, DT == 64 && KG == 1 ? 3 : 2) void pa
   }
 
   const float slope = ALIBI ? (live ? p.alibi_slopes[hq] * kLog2eF : 0.0f) : 0.0f;
+  // Where no row sees a key behind it the distance needs no absolute value and the bias goes
+  // into the product's scaling (16384 tokens 2.46 -> 2.36 ms); its parts stay finite.
+  const bool linear = ALIBI && !CAP && p.causal && !p.prefix_lens && __all(fabsf(slope) < 1e25f);
 
   // ---- tile copies: load i of thread tid fills unit 256 i + tid of the tile, of row
   // i kThreads / UPR + tid / UPR
@@ -355,9 +358,7 @@ __global__ __launch_bounds__(KG * kThreads, DT == 64 && KG == 1 ? 3 : 2) void pa
         auto put = [&](int i, float x) { s[i / 16][i % 16] = fmaf(-slope, fabsf(gap - offset(i)), x); };
         if constexpr (CAP) {
           each_score<16 * KB>(rule, get, put);
-        } else if (p.causal && !p.prefix_lens) {
-          // no row sees a key behind it, so the distance needs no absolute value and the bias
-          // goes into the product's scaling: 16384 tokens 2.46 -> 2.36 ms
+        } else if (linear) {
           const float base = -slope * gap;
 #pragma unroll
           for (int i = 0; i < 16 * KB; ++i) s[i / 16][i % 16] = fmaf(get(i), rule.scale, fmaf(slope, offset(i), base));

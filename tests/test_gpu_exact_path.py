@@ -909,3 +909,19 @@ def test_the_largest_page_step(dev):
     want = (2 ** 31 - 1) * bs + 70000 - bs
     assert step.slot_mapping.view(n, 3).tolist() == [[want, want + 1, want + 2]] * n
     assert step.status.tolist() == [0, 0] and int(step.query_start_loc[-1]) == 3 * n
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(causal=False), dict(prefix=[40, 200, 1]), dict(window=50),
+                                dict(prefix=[3, 150, 90], window=20, cap=30.0)])
+def test_packed_biases_in_every_mask(dev, kw):
+    """Keys behind a row, which prefixes and full masks show it, are biased by their distance too."""
+    _check_packed(dev, [100, 260, 91], 4, 2, 128, torch.bfloat16, slopes=torch.tensor([0.6, 0.1, -0.05, 0.0], device=dev),
+                  **kw)
+
+
+@pytest.mark.parametrize("slope", [1e4, 1e24, 1e30, 1e37])
+def test_packed_steep_biases(dev, slope):
+    """A bias that leaves a row nothing but its own key: its value, bit for bit."""
+    q, k, v = _qkv(dev, 300, 2, 1, 64, torch.bfloat16, 52)
+    out = S.compute_packed_attention(q, k, v, _starts([300], dev), alibi_slopes=torch.full((2,), slope, device=dev))
+    assert torch.equal(out, v.expand(-1, 2, -1))
